@@ -135,6 +135,11 @@ SIGNATURES = [
     ("tca_emit_hipcc_argc", _U32, [_P]),
     ("tca_emit_hipcc_arg", _STR, [_P, _U32]),
     ("tca_emit_free", None, [_P]),
+    # operator programs (tca_op.h)
+    ("tca_op_emit", _c.c_int, [_STR, _STR, _STR, _c.POINTER(_P)]),
+    ("tca_op_program_name", _STR, [_P]),
+    ("tca_op_last_error", _STR, []),
+    ("tca_op_list", _STR, []),
     # .tca frontend (tca_syntax.h)
     ("tca_syntax_parse_module", _c.c_int, [_STR, _c.POINTER(_P)]),
     ("tca_syntax_parse_source", _c.c_int, [_STR, _STR, _I32, _c.POINTER(_P)]),

@@ -27,6 +27,8 @@ SOURCES = [
     "cg/emit_hip.cpp",
     "cg/gemm_emit.cpp",
     "cg/capi.cpp",
+    "cg/operators.cpp",
+    "cg/op_capi.cpp",
     "syntax/lexer.cpp",
     "syntax/parser.cpp",
     "syntax/check.cpp",
@@ -80,11 +82,11 @@ def build_kernels(jobs=8, force=False, extra=()):
     """Emits and compiles every registered program, plus `extra` (name,
     factory, flags) triples such as the test suite's generated programs,
     into _kcache/; code objects of neither are pruned."""
-    from . import compiler, programs
+    from . import compiler, operators, programs
 
     jobs_list = []
     current = set()
-    for name, factory, flags in list(programs.all_builds()) + list(extra):
+    for name, factory, flags in list(programs.all_builds()) + operators.all_builds() + list(extra):
         prog = factory()
         emitted = prog.emit(flags=flags)
         key = compiler.cache_key(emitted.source, emitted.hipcc)

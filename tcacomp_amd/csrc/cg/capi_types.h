@@ -23,6 +23,7 @@ struct tca_builder_s {
 
 struct tca_emit_result_s {
   tca::cg::Result r;
+  std::string program;  // an operator program's name (tca_op.h)
 };
 
 #endif  // TCA_CG_CAPI_TYPES_H_

@@ -1,0 +1,405 @@
+// product.h — 16-bit matrix products of a dense sublayer (family P): a
+// projection with bias, activation and residual in its epilogue, two
+// projections whose results meet in the epilogue (gated), and the gradients
+// of both.
+//
+//   C[m, n] = sum_k A[m, k] B[k, n], 32-bit sums on the matrix cores
+//   (v_mfma_f32_16x16x32), rounded once when the epilogue stores
+//
+// An operand is K-contiguous (rows of k, as x [M][K] in a forward product) or
+// row-contiguous (rows of its own index, as a weight [K][N]; as x and dz in
+// dW = x^T dz, whose reduction runs over their rows). The B side of a tile has
+// two halves. In a plain product they are neighbouring columns of one matrix;
+// in a pair (PAIR) the same columns of two matrices, so that a lane holds both
+// products of an output element and the epilogue combines them. A product
+// may run over two segments of k (SEGS), each with its own pair of operands:
+// dx = dg Wg^T + du Wu^T is one chain of sums.
+#ifndef TCA_HIP_PRODUCT_H_
+#define TCA_HIP_PRODUCT_H_
+
+#include "tca/hip/gemm.h"
+#include "tca/hip/rows.h"
+
+namespace tca {
+namespace hip {
+
+// ----------------------------------------------------------- activations
+// Results are rounded to 16 bits by every caller, so the hardware's exp2 and
+// reciprocal (1 ulp each) stand in for the rounded ones.
+enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
+
+__device__ __forceinline__ float act_sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
+}
+// Phi(z), the normal distribution: erfc keeps its relative precision at -z.
+__device__ __forceinline__ float act_phi(float z) { return 0.5f * erfcf(-0.70710678118654752f * z); }
+
+template <int ACT>
+__device__ __forceinline__ float act(float z) {
+  if constexpr (ACT == kActRelu) return z < 0.0f ? 0.0f : z;
+  else if constexpr (ACT == kActSilu) return z * act_sigmoid(z);
+  else if constexpr (ACT == kActGelu) return z * act_phi(z);
+  else if constexpr (ACT == kActGeluTanh)  // 1 + tanh(u) = 2 sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3)
+    return z * act_sigmoid(1.59576912160573071f * z * __builtin_fmaf(0.044715f * z, z, 1.0f));
+  else return z;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if constexpr (ACT == kActRelu) {
+    return z <= 0.0f ? 0.0f : 1.0f;
+  } else if constexpr (ACT == kActSilu) {
+    const float s = act_sigmoid(z);
+    return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
+  } else if constexpr (ACT == kActGelu) {
+    return act_phi(z) + z * (0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z));
+  } else if constexpr (ACT == kActGeluTanh) {
+    const float s = act_sigmoid(1.59576912160573071f * z * __builtin_fmaf(0.044715f * z, z, 1.0f));
+    const float du = 1.59576912160573071f * __builtin_fmaf(3.0f * 0.044715f * z, z, 1.0f);
+    return s * __builtin_fmaf(z * du, 1.0f - s, 1.0f);
+  } else {
+    return 1.0f;
+  }
+}
+
+// ------------------------------------------------------------- epilogues
+// Each takes four consecutive columns n .. n + 3 of row m < M, n < N, and
+// stores those before N.
+template <typename T>
+__device__ __forceinline__ f32x4_t load4(const T* p, uint32_t n, uint32_t N) {
+  f32x4_t f;
+  if (n + 4u <= N) {
+    const vec<T, 4> v = load_vec_any<T, 4, false>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = static_cast<float>(v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = n + e < N ? static_cast<float>(p[e]) : 0.0f;
+  }
+  return f;
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, uint32_t n, uint32_t N, f32x4_t f) {
+  if (n + 4u <= N) {
+    vec<T, 4> v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v.set(e, static_cast<T>(f[e]));
+    store_vec_any<T, 4, false>(p, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < N) p[e] = static_cast<T>(f[e]);
+  }
+}
+
+// y = res + act(z), z = v + b [z stored too]. res may be y: an element is
+// read by the lane that then writes it.
+template <typename T, int ACT, bool BIAS, bool RES, bool SAVE>
+struct LinearStore {
+  const T* b;
+  const T* res;
+  T* y;
+  T* z;
+  uint32_t N;
+  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, f32x4_t v) const {
+    const uint64_t at = static_cast<uint64_t>(m) * N + n;
+    if constexpr (BIAS) v += load4(b + n, n, N);
+    if constexpr (SAVE) store4(z + at, n, N, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = act<ACT>(v[e]);
+    if constexpr (RES) v += load4(res + at, n, N);
+    store4(y + at, n, N, v);
+  }
+};
+// h = act(g) u, g = v0 + bg, u = v1 + bu [g and u stored too].
+template <typename T, int ACT, bool BIAS, bool SAVE>
+struct GatedStore {
+  const T* bg;
+  const T* bu;
+  T* h;
+  T* g;
+  T* u;
+  uint32_t N;
+  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, f32x4_t v0, f32x4_t v1) const {
+    const uint64_t at = static_cast<uint64_t>(m) * N + n;
+    if constexpr (BIAS) {
+      v0 += load4(bg + n, n, N);
+      v1 += load4(bu + n, n, N);
+    }
+    if constexpr (SAVE) {
+      store4(g + at, n, N, v0);
+      store4(u + at, n, N, v1);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v0[e] = act<ACT>(v0[e]) * v1[e];
+    store4(h + at, n, N, v0);
+  }
+};
+// The results themselves: of one product, or of a pair.
+template <typename T>
+struct PlainStore {
+  T* c;
+  T* c1;
+  uint32_t N;
+  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, f32x4_t v) const {
+    store4(c + static_cast<uint64_t>(m) * N + n, n, N, v);
+  }
+  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, f32x4_t v0, f32x4_t v1) const {
+    store4(c + static_cast<uint64_t>(m) * N + n, n, N, v0);
+    store4(c1 + static_cast<uint64_t>(m) * N + n, n, N, v1);
+  }
+};
+
+// ------------------------------------------------------------- operands
+// M x N results over SEGS segments of K. a[s]: [M][K] or, A_RC, [K][M]; b[h][s]
+// [N][K] or, B_RC, [K][N], b[1] the second matrix of a pair. Rows are packed.
+template <int SEGS>
+struct Operands {
+  const uint16_t* a[SEGS];
+  const uint16_t* b[2][SEGS];
+  uint32_t M, N, K;
+};
+
+// n <= 8 values at p, zeros after them.
+__device__ __forceinline__ u32x4 gather16(const uint16_t* p, uint32_t n) {
+  uint64_t lo = 0u, hi = 0u;
+#pragma unroll 1
+  for (uint32_t e = 0; e < n; ++e) {
+    const uint64_t v = p[e];
+    if (e < 4u) lo |= v << (16u * e);
+    else hi |= v << (16u * (e - 4u));
+  }
+  return u32x4{static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
+               static_cast<uint32_t>(hi >> 32)};
+}
+
+// ------------------------------------- any shape, any alignment: 128x128 tiles
+// 4 waves of 64x64 (of a pair: 64x32 of each product), 64-deep slices of K,
+// global memory -> registers (16 bytes a lane, unguarded: rows and chunks past
+// the end re-read the last ones) -> LDS (two buffers, one barrier a slice).
+// A chunk that runs past the end of its row is loaded from 8 elements before
+// that end and moved into place, so the tail of k adds zeros.
+template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, typename Epi>
+__device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& epi, uint32_t tile) {
+  constexpr uint32_t BM = 128, HB = 64, SLICE = BM * 64u, HALF = HB * 64u, BUF = SLICE + 2u * HALF;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * BUF];
+  const uint32_t M = p.M, N = p.N, K = p.K, width = PAIR ? HB : 2u * HB;
+  uint32_t tm, tn;
+  gemm_tile_coords((M - 1u) / BM + 1u, (N - 1u) / width + 1u, &tm, &tn, tile);
+  const uint32_t m0 = tm * BM, n0 = tn * width;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t wm = (wave >> 1) * 64u, wn = (wave & 1u) * 32u;
+
+  // One chunk of 8 of a K-contiguous panel row, or of row k of a row-contiguous
+  // panel of W columns, and its place in a slice.
+  auto kc_load = [&](const uint16_t* base, uint32_t row, uint32_t rows, uint32_t k) -> u32x4 {
+    const uint16_t* r = base + static_cast<uint64_t>(row < rows ? row : rows - 1u) * K;
+    if (K < 8u) return gather16(r + k, k < K ? K - k : 0u);
+    return load16_any(r + (k < K - 8u ? k : K - 8u));
+  };
+  auto kc_fix = [&](u32x4 v, uint32_t k) -> u32x4 {
+    return K < 8u || k + 8u <= K ? v : shift_down16(v, k - (K - 8u));
+  };
+  auto rc_load = [&](const uint16_t* base, uint32_t c, uint32_t cols, uint32_t k) -> u32x4 {
+    const uint16_t* r = base + static_cast<uint64_t>(k < K ? k : K - 1u) * cols;
+    if (cols < 8u) return gather16(r + (c < cols ? c : 0u), c < cols ? cols - c : 0u);
+    return load16_any(r + (c < cols - 8u ? c : cols - 8u));
+  };
+  auto rc_fix = [&](u32x4 v, uint32_t c, uint32_t cols, uint32_t k) -> u32x4 {
+    if (k >= K) return u32x4{0u, 0u, 0u, 0u};
+    return cols < 8u || c + 8u <= cols ? v : shift_down16(v, c - (cols - 8u));
+  };
+  u32x4 ra[4], rb[2][2];
+  const uint32_t ns = (K + 63u) / 64u, total = ns * SEGS;
+  auto load = [&](uint32_t t) {
+    const uint32_t seg = SEGS == 1 || t < ns ? 0u : 1u, k0 = (t - seg * ns) * 64u;
+    const uint16_t* a = SEGS == 1 || seg == 0u ? p.a[0] : p.a[SEGS - 1];
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+      const uint32_t c = i * 256u + tid;
+      ra[i] = A_RC ? rc_load(a, m0 + (c & 15u) * 8u, M, k0 + (c >> 4)) : kc_load(a, m0 + (c >> 3), M, k0 + (c & 7u) * 8u);
+    }
+#pragma unroll
+    for (uint32_t h = 0; h < 2u; ++h) {
+      const uint32_t hp = PAIR ? h : 0u, nh = PAIR ? n0 : n0 + HB * h;
+      const uint16_t* b = SEGS == 1 || seg == 0u ? p.b[hp][0] : p.b[hp][SEGS - 1];
+#pragma unroll
+      for (uint32_t i = 0; i < 2u; ++i) {
+        const uint32_t c = i * 256u + tid;
+        rb[h][i] = B_RC ? rc_load(b, nh + (c & 7u) * 8u, N, k0 + (c >> 3)) : kc_load(b, nh + (c >> 3), N, k0 + (c & 7u) * 8u);
+      }
+    }
+  };
+  auto write = [&](uint32_t t) {
+    const uint32_t k0 = (SEGS == 1 || t < ns ? t : t - ns) * 64u;
+    uint16_t* As = lds + (t & 1u) * BUF;
+    const bool ktail = k0 + 64u > K;
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+      const uint32_t c = i * 256u + tid;
+      if constexpr (A_RC) {
+        const uint32_t k = c >> 4, m = (c & 15u) * 8u;
+        if (ktail || m0 + BM > M) ra[i] = rc_fix(ra[i], m0 + m, M, k0 + k);
+        *reinterpret_cast<u32x4*>(&As[swz_kn<BM>(k, m)]) = ra[i];
+      } else {
+        if (ktail) ra[i] = kc_fix(ra[i], k0 + (c & 7u) * 8u);
+        *reinterpret_cast<u32x4*>(&As[swz_rows64(c >> 3, c & 7u)]) = ra[i];
+      }
+    }
+#pragma unroll
+    for (uint32_t h = 0; h < 2u; ++h) {
+      uint16_t* Bs = As + SLICE + h * HALF;
+      const uint32_t nh = PAIR ? n0 : n0 + HB * h;
+#pragma unroll
+      for (uint32_t i = 0; i < 2u; ++i) {
+        const uint32_t c = i * 256u + tid;
+        if constexpr (B_RC) {
+          const uint32_t k = c >> 3, n = (c & 7u) * 8u;
+          if (ktail || nh + HB > N) rb[h][i] = rc_fix(rb[h][i], nh + n, N, k0 + k);
+          *reinterpret_cast<u32x4*>(&Bs[swz_kn<HB>(k, n)]) = rb[h][i];
+        } else {
+          if (ktail) rb[h][i] = kc_fix(rb[h][i], k0 + (c & 7u) * 8u);
+          *reinterpret_cast<u32x4*>(&Bs[swz_rows64(c >> 3, c & 7u)]) = rb[h][i];
+        }
+      }
+    }
+  };
+  f32x4_t acc[2][4][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[h][i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  auto compute = [&](uint32_t t) {
+    const uint16_t* As = lds + (t & 1u) * BUF;
+#pragma unroll
+    for (uint32_t s = 0; s < 2u; ++s) {
+      bf16x8 fa[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 4u; ++i) {
+        if constexpr (A_RC) fa[i] = frag_b16_tr<BM>(As, wm + 16u * i, lane, 32u * s);
+        else fa[i] = *reinterpret_cast<const bf16x8*>(&As[swz_rows64(wm + 16u * i + (lane & 15u), 4u * s + (lane >> 4))]);
+      }
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) {
+        const uint16_t* Bs = As + SLICE + h * HALF;
+#pragma unroll
+        for (uint32_t j = 0; j < 2u; ++j) {
+          bf16x8 fb;
+          if constexpr (B_RC) fb = frag_b16_tr<HB>(Bs, wn + 16u * j, lane, 32u * s);
+          else fb = *reinterpret_cast<const bf16x8*>(&Bs[swz_rows64(wn + 16u * j + (lane & 15u), 4u * s + (lane >> 4))]);
+          // Operands swapped: a lane ends with four consecutive columns of one row.
+#pragma unroll
+          for (uint32_t i = 0; i < 4u; ++i) acc[h][i][j] = mfma_16x16x32_16b<F16>(fb, fa[i], acc[h][i][j]);
+        }
+      }
+    }
+  };
+  if (total > 0u) {
+    load(0u);
+    write(0u);
+    __syncthreads();
+    for (uint32_t t = 0; t < total; ++t) {
+      if (t + 1u < total) load(t + 1u);
+      compute(t);
+      if (t + 1u < total) write(t + 1u);
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 4u; ++i) {
+    const uint32_t m = m0 + wm + 16u * i + (lane & 15u);
+    if (m >= M) continue;
+#pragma unroll
+    for (uint32_t j = 0; j < 2u; ++j) {
+      const uint32_t n = n0 + wn + 16u * j + 4u * (lane >> 4);
+      if constexpr (PAIR) {
+        if (n < N) epi(m, n, acc[0][i][j], acc[1][i][j]);
+      } else {
+        if (n < N) epi(m, n, acc[0][i][j]);
+        if (n + HB < N) epi(m, n + HB, acc[1][i][j]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------ gradients of the pre-activations
+// One element each: dz = dy act'(z) of a projection, dg = dh u act'(g) and
+// du = dh act(g) of a gated pair. i(e) is (dy, z) or (dh, g, u).
+template <typename T, int ACT, bool GATED>
+struct Slope {
+  const T* dy;
+  const T* z;  // g of a pair
+  const T* u;
+  T* dz;  // dg of a pair; no store where ACT is none
+  T* du;
+  // The vector at `at` (its E values before `end`): f0 = dz or dg, f1 = du.
+  template <int E>
+  __device__ __forceinline__ void operator()(uint64_t at, uint32_t c, uint32_t C, float (&f0)[E], float (&f1)[E]) const {
+    float a[E], b[E], d[E];
+    row_load<E>(dy + at, c, C, d);
+    if constexpr (ACT != kActNone || GATED) row_load<E>(z + at, c, C, a);
+    if constexpr (GATED) row_load<E>(u + at, c, C, b);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if constexpr (GATED) {
+        f0[e] = d[e] * b[e] * act_slope<ACT>(a[e]);
+        f1[e] = d[e] * act<ACT>(a[e]);
+      } else if constexpr (ACT != kActNone) {
+        f0[e] = d[e] * act_slope<ACT>(a[e]);
+      } else {
+        f0[e] = d[e];
+      }
+    }
+    if constexpr (GATED || ACT != kActNone) row_store<E>(dz + at, c, C, f0);
+    if constexpr (GATED) row_store<E>(du + at, c, C, f1);
+  }
+};
+
+// Over the whole plane as one row of `n` elements, 8 a lane.
+template <typename T, int ACT, bool GATED>
+__device__ __forceinline__ void slope_flat(const Slope<T, ACT, GATED>& f, uint32_t n) {
+  const uint32_t c = (blockIdx.x * 256u + threadIdx.x) * 8u;
+  if (c >= n) return;
+  float f0[8], f1[8];
+  f(0u, c, n, f0, f1);
+}
+
+// ... with the column sums of a bias' gradient, of the values before they are
+// rounded: 512 columns by 4 rows a workgroup, over row chunk p of P; `part`
+// is [P][1 + GATED][N].
+template <typename T, int ACT, bool GATED>
+__device__ __forceinline__ void slope_columns(const Slope<T, ACT, GATED>& f, float* __restrict__ part, uint32_t M,
+                                              uint32_t N, uint32_t P) {
+  __shared__ float join[4][512];
+  const uint32_t p = blockIdx.x % P, c0 = blockIdx.x / P * 512u, c = c0 + lane_id() * 8u, slot = wave_id();
+  const uint64_t rows = (M - 1u) / P + 1u, first = p * rows, last = first + rows < M ? first + rows : M;
+  float s0[8], s1[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s0[e] = s1[e] = 0.0f;
+  if (c < N)
+    for (uint64_t r = first + slot; r < last; r += 4u) {
+      float f0[8], f1[8];
+      f(r * N, c, N, f0, f1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s0[e] += f0[e];
+        if constexpr (GATED) s1[e] += f1[e];
+      }
+    }
+  constexpr uint32_t Q = GATED ? 2u : 1u;
+#pragma unroll
+  for (uint32_t q = 0; q < Q; ++q) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) join[slot][lane_id() * 8u + e] = q == 0u ? s0[e] : s1[e];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < 512u && c0 + i < N; i += 256u)
+      part[(static_cast<uint64_t>(p) * Q + q) * N + c0 + i] = ((join[0][i] + join[1][i]) + join[2][i]) + join[3][i];
+  }
+}
+
+}  // namespace hip
+}  // namespace tca
+
+#endif  // TCA_HIP_PRODUCT_H_

@@ -156,16 +156,22 @@ class Program:
                         target.encode() if target else None, flags, ctypes.byref(out))
         if rc != 0:
             raise BuildError(L.tca_builder_error(self.b._h).decode())
-        try:
-            n = L.tca_emit_hipcc_argc(out)
-            return EmitResult(
-                source=L.tca_emit_source(out).decode(),
-                plan=L.tca_emit_plan(out).decode(),
-                report=L.tca_emit_report(out).decode(),
-                hipcc=[L.tca_emit_hipcc_arg(out, i).decode() for i in range(n)],
-            )
-        finally:
-            L.tca_emit_free(out)
+        return _take_result(out)
+
+
+def _take_result(out):
+    """The EmitResult of a tca_emit_result handle, which is freed."""
+    L = _lib.lib()
+    try:
+        n = L.tca_emit_hipcc_argc(out)
+        return EmitResult(
+            source=L.tca_emit_source(out).decode(),
+            plan=L.tca_emit_plan(out).decode(),
+            report=L.tca_emit_report(out).decode(),
+            hipcc=[L.tca_emit_hipcc_arg(out, i).decode() for i in range(n)],
+        )
+    finally:
+        L.tca_emit_free(out)
 
 
 class EmitResult:

@@ -1,0 +1,167 @@
+"""The operator programs without a GPU: the definitions the GPU tests use
+against differences and autograd, the emitted programs, which kernel a size
+takes, and the refusals of the C ABI."""
+import ctypes
+import itertools
+
+import pytest
+import torch
+
+import operators_ref as ref
+from tcacomp_amd import _lib, compiler, operators
+from tcacomp_amd.compiler import TensorDesc
+from tcacomp_amd.pkg import TBF16, BuildError
+
+ELEM_CODES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+def desc(elem, *shape):
+    return TensorDesc(16, shape, ELEM_CODES[elem])
+
+
+def compiled(op):
+    """Emission and plan only: no code object is needed."""
+    return compiler.CompiledProgram(op.name, op.emit(), "")
+
+
+# ------------------------------------------------------------ definitions
+
+@pytest.mark.parametrize("name", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_slopes_against_differences(name):
+    z = torch.linspace(-6, 6, 241, dtype=torch.float64) + 0.0125  # no point at relu's corner
+    d = 1e-6
+    diff = (ref.act(name, z + d) - ref.act(name, z - d)) / (2 * d)
+    # the difference's own error: d^2 / 6 of a third derivative below 3, and its cancellation
+    assert (ref.slope(name, z) - diff).abs().max() <= d * d + 8 * 2.0 ** -53 / d * 7
+
+
+def test_layer_norm_gradients_against_differences_and_autograd():
+    torch.manual_seed(0)
+    x, gamma, beta, dy, dres = (torch.randn(s, dtype=torch.float64) for s in ((3, 5), (5,), (5,), (3, 5), (3, 5)))
+    _, mean, rstd = ref.layer_norm(x, gamma, beta, 1e-5)
+    dx, dg, db = ref.layer_norm_backward(dy, x, gamma, mean, rstd, dres)
+    leaves = [t.clone().requires_grad_() for t in (x, gamma, beta)]
+    ((ref.layer_norm(*leaves, 1e-5)[0] * dy).sum() + (leaves[0] * dres).sum()).backward()
+    for got, leaf in zip((dx, dg, db), leaves):
+        assert torch.allclose(got, leaf.grad, rtol=1e-10, atol=1e-10)
+    f = lambda v: (ref.layer_norm(v, gamma, beta, 1e-5)[0] * dy).sum() + (v * dres).sum()  # noqa: E731
+    for i, j in itertools.product(range(3), range(5)):
+        e = torch.zeros_like(x)
+        e[i, j] = 1e-5
+        assert abs(float((f(x + e) - f(x - e)) / 2e-5 - dx[i, j])) < 1e-6
+
+
+# --------------------------------------------------------------- emission
+
+def test_attributes_in_any_order_are_one_program():
+    L = _lib.lib()
+    seen = set()
+    for words in itertools.permutations(["elem=bf16", "act=gelu", "bias", "save"]):
+        out = ctypes.c_void_p()
+        assert L.tca_op_emit(b"linear", " ".join(words).encode(), None, ctypes.byref(out)) == 0
+        seen.add((L.tca_op_program_name(out), L.tca_emit_plan(out), L.tca_emit_source(out)))
+        L.tca_emit_free(out)
+    assert len(seen) == 1
+
+
+def test_elements_by_name_or_type():
+    assert operators.gated(TBF16).name == operators.gated("bf16").name == "gated_bf16_silu"
+    assert operators.layer_norm("bf16", weight="bf16").name == operators.layer_norm("bf16").name
+
+
+def test_every_operator_is_listed_and_built():
+    listed = operators.list_operators()
+    assert set(listed) == {"layer_norm", "layer_norm_backward", "linear", "linear_backward", "gated", "gated_backward"}
+    built = [f() for _, f, _ in operators.all_builds()]
+    assert {o.op for o in built} == set(listed)
+    assert len({o.name for o in built}) == len(built)
+
+
+@pytest.mark.parametrize("op,attributes,word", [
+    ("linear", "elem=f32", "elem=f32"), ("linear", "", "no elem"), ("linear", "elem=bf16 act=swish", "act=swish"),
+    ("linear", "elem=bf16 stats", "stats"), ("linear", "elem=bf16 bias=1", "bias=1"), ("linear", "elem=bf16 elem=f16", "twice"),
+    ("gated", "elem=bf16 residual", "residual"), ("gated_backward", "elem=bf16 save", "save"), ("linear", "elem=bf16 act", "act"),
+    ("layer_norm", "elem=bf16 act=gelu", "act=gelu"), ("layer_norm", "elem=bf16 weight=f16", "weight=f16"),
+    ("layer_norm", "elem=u8", "elem=u8"), ("linear_backward", "elem=bf16 residual", "residual")])
+def test_refused_attributes(op, attributes, word):
+    with pytest.raises(BuildError, match=word):
+        operators.Operator(op, attributes)
+
+
+def test_refusals_of_the_c_entry():
+    L = _lib.lib()
+    out = ctypes.c_void_p(7)
+    assert L.tca_op_emit(None, b"elem=bf16", None, ctypes.byref(out)) == _lib.TCA_ERR_INVALID
+    assert L.tca_op_emit(b"linear", b"elem=bf16", None, None) == _lib.TCA_ERR_INVALID
+    assert L.tca_op_emit(b"conv", b"elem=bf16", None, ctypes.byref(out)) == _lib.TCA_ERR_NOT_FOUND
+    assert out.value is None and b"no operator conv" in L.tca_op_last_error()
+    assert L.tca_op_emit(b"linear", b"elem=bf16", b"gfx942", ctypes.byref(out)) == _lib.TCA_ERR_UNSUPPORTED
+    assert b"gfx942" in L.tca_op_last_error()
+    assert L.tca_op_emit(b"linear", None, None, ctypes.byref(out)) == _lib.TCA_ERR_UNSUPPORTED
+    assert L.tca_op_program_name(None) is None
+    with pytest.raises(BuildError, match="emit flags"):
+        operators.linear("bf16").emit(flags=1)
+
+
+# ------------------------------------------- which kernels a size takes
+
+def norm_tensors(elem, R, C):
+    return [desc(elem, R, C), desc(elem, C), desc(elem, C), desc(elem, R, C)]
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+def test_every_row_length_takes_one_norm_kernel(elem):
+    p = compiled(operators.layer_norm(elem))
+    lengths = sorted({c + d for e in range(3, 18) for c in (1 << e,) for d in (-1, 0, 1)} | {0, 1, 2, 100001})
+    for C in lengths:
+        assert len(p.selected_symbols(norm_tensors(elem, 3, C))) == 1, C
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+def test_every_row_length_takes_one_norm_backward_kernel(elem):
+    p = compiled(operators.layer_norm_backward(elem))
+    for C in sorted({c + d for e in range(3, 18) for c in (1 << e,) for d in (-1, 0, 1)} | {1, 2, 100001}):
+        for R in (1, 5, 4000):
+            t = [desc(elem, R, C), desc(elem, R, C), desc(elem, C), desc("f32", R), desc("f32", R), desc(elem, R, C),
+                 desc(elem, C), desc(elem, C)]
+            names = p.selected_symbols(t)
+            assert [n.endswith("join") for n in names].count(True) == 1 and len(names) in (2, 3), (R, C, names)
+
+
+def selected(p, tensors):
+    """{symbol: grid} of the kernels a launch with these tensors runs."""
+    L = _lib.lib()
+    syms = p.kernel_symbols()
+    out, grids = (ctypes.c_uint8 * len(syms))(), (ctypes.c_uint64 * len(syms))()
+    fd = (ctypes.c_uint32 * 1)()
+    _lib.check(L.tca_program_selected(p.parsed(), compiler._descriptors(tensors), len(tensors), fd, 0, out, grids, None, len(syms)))
+    return {s: g for s, f, g in zip(syms, out, grids) if f and g}
+
+
+def test_partial_rows_are_as_many_as_the_join_adds():
+    """partial_rows on the device restates the grid of the kernel that writes
+    the partial rows."""
+    p = compiled(operators.layer_norm_backward("bf16"))
+    for R, C in itertools.product((1, 3, 4, 5, 63, 64, 65, 255, 256, 257, 1023, 1024, 1025, 100000), (64, 300, 1000, 2000, 4000, 8000, 16000, 20000)):
+        t = [desc("bf16", R, C), desc("bf16", R, C), desc("bf16", C), desc("f32", R), desc("f32", R), desc("bf16", R, C),
+             desc("bf16", C), desc("bf16", C)]
+        grids = selected(p, t)
+        if C > 16384:
+            parts = min(-(-R // 64), 32)
+            assert grids["tca_" + p.name + "_columns"] == -(-C // 512) * parts
+        else:
+            (lanes, grid), = [(int(s.rsplit("_", 1)[1].split("x")[0]), g) for s, g in grids.items() if not s.endswith("join")]
+            assert grid == min(-(-R // (1024 // lanes)), 256)
+
+
+def test_shape_contract():
+    p = compiled(operators.gated("bf16", save=True))
+    good = [desc("bf16", 4, 8), desc("bf16", 8, 16), desc("bf16", 8, 16)] + [desc("bf16", 4, 16)] * 3
+    assert p.check(good) == 0
+    for i, bad in ((1, desc("bf16", 9, 16)), (2, desc("bf16", 8, 17)), (3, desc("bf16", 5, 16)), (4, desc("f16", 4, 16)),
+                   (0, desc("bf16", 4, 8, 1))):
+        t = list(good)
+        t[i] = bad
+        assert p.check(t) == _lib.TCA_ERR_SHAPE
+    assert p.check(good[:-1]) == _lib.TCA_ERR_INVALID
+    assert p.check([TensorDesc(8, (4, 8), 2)] + good[1:]) == _lib.TCA_ERR_INVALID
