@@ -359,14 +359,39 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   }
   ops << "  p.M = " << p.M << ";\n  p.N = " << p.N << ";\n  p.K = " << p.K << ";\n  const auto epi = " << p.epi << ";\n";
   const std::string f16 = Bool(a.elem == "f16");
-  const std::string targs = "<" + f16 + ", " + Bool(p.a_rc) + ", " + Bool(p.b_rc) + ", " + Bool(p.pair) + ", " + std::to_string(p.segs) + ">";
-  Writer::Kernel k;
-  k.suffix = p.suffix;
-  k.params = p.params;
-  k.body = ops.str() + "  tca::hip::product_any" + targs + "(p, epi, blockIdx.x);\n";
-  k.grid = p.M + "/128 " + p.N + (p.pair ? "/64" : "/128");
-  k.detail = p.what + ", tiles of 128x128, any shape and alignment";
-  w->Add(k);
+  auto add = [&](const std::string& suffix, const std::string& call, uint32_t block, uint32_t rows, uint32_t cols,
+                 const std::vector<std::string>& records, const std::string& detail) {
+    Writer::Kernel k;
+    k.suffix = p.suffix + suffix;
+    k.params = p.params;
+    k.block = block;
+    k.body = ops.str() + "  tca::hip::" + call + "(p, epi, blockIdx.x);\n";
+    k.grid = p.M + "/" + std::to_string(rows) + " " + p.N + "/" + std::to_string(p.pair ? cols / 2u : cols);
+    k.records = records;
+    k.detail = p.what + ", " + detail;
+    w->Add(k);
+  };
+  const std::string targs = f16 + ", " + Bool(p.a_rc) + ", " + Bool(p.b_rc) + ", " + Bool(p.pair) + ", " + std::to_string(p.segs);
+  // Rows of whole 16-byte chunks, of both operands, go straight into LDS.
+  std::vector<std::string> whole;
+  for (const std::string& d : {p.a_rc ? p.M : p.K, p.b_rc ? p.N : p.K})
+    if (whole.empty() || whole[0] != d) whole.push_back(d);
+  std::vector<std::string> aligned, odd;
+  for (const auto& d : whole) {
+    aligned.push_back(When(d, 0, kMost, 8));
+    odd.push_back("unless " + d + " 0 " + std::to_string(kMost) + " 8 0");
+  }
+  const std::string plane = p.M + "*" + p.N;
+  const uint64_t kLarge = (p.pair ? 32768ull : 65536ull) * 192u, kAll = 18446744073709551615ull;
+  auto with = [](std::vector<std::string> v, const std::string& r) {
+    v.push_back(r);
+    return v;
+  };
+  add("_l", "product_ring<" + targs + ", 256, 128, 2, 4>", 512, 256, 256, with(aligned, When(plane, kLarge, kAll)),
+      "tiles of 256x256, 8 waves, direct to LDS");
+  add("_s", "product_ring<" + targs + ", 128, 64, 2, 2>", 256, 128, 128, with(aligned, When(plane, 0, kLarge - 1u)),
+      "tiles of 128x128, 4 waves, direct to LDS");
+  add("", "product_any<" + targs + ">", 256, 128, 128, odd, "tiles of 128x128, any shape and alignment");
 }
 
 void EmitForward(const Attrs& a, bool gated, Writer* w) {

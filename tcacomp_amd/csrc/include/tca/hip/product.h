@@ -323,6 +323,200 @@ __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& 
   }
 }
 
+// ------------------------- rows of whole 16-byte chunks: straight into LDS
+// What chunks that lie outside an operand read (a static constant of the code
+// object): rows past the end and slices past the last add zeros to the sums.
+static __device__ __attribute__((aligned(16))) const uint32_t kZeroChunk[4] = {0u, 0u, 0u, 0u};
+
+// A tile of BM x 2 HB (a pair: BM x HB of each product), WGM x WGN waves, each
+// (BM / WGM) rows by HB / WGN columns of either half, for operands whose rows
+// are whole chunks of 8 (K % 8 == 0 where K-contiguous, M or N % 8 == 0 where
+// row-contiguous).
+//
+// K advances in 32-deep slices through a ring of 4 slots of LDS, filled by
+// global_load_lds (lane i of a load writes 16 bytes at 16 i of a 1 KiB chunk,
+// from any global address: each lane's address is the inverse of the LDS
+// swizzle). Step t waits until slice t + 1 has landed and every read of slice
+// t has completed, one barrier, then runs the MFMAs of slice t on registers
+// while it reads the fragments of slice t + 1 into the other register set and
+// loads slice t + 4 into slice t's slot. Every step issues the same loads: a
+// chunk outside its operand, or past the last slice, is read from kZeroChunk,
+// so no tail of k, edge of the plane or border between segments needs code
+// of its own, and the count of loads in flight is static. (The operands are
+// __restrict__ parameters: without them the compiler takes a transposing read
+// of LDS to depend on every load into it and waits for all of them.)
+template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, uint32_t HB, uint32_t WGM, uint32_t WGN, typename Epi>
+__device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0, const uint16_t* __restrict__ pa1,
+                                                const uint16_t* __restrict__ pb00, const uint16_t* __restrict__ pb01,
+                                                const uint16_t* __restrict__ pb10, const uint16_t* __restrict__ pb11,
+                                                const uint16_t* __restrict__ zero, uint32_t M, uint32_t N, uint32_t K,
+                                                const Epi& epi, uint32_t tile) {
+  constexpr uint32_t WAVES = WGM * WGN, TM = BM / WGM, TH = HB / WGN, ASL = BM * 32u, BSL = HB * 32u, SLOT = ASL + 2u * BSL;
+  constexpr int IM = TM / 16, JH = TH / 16, JN = 2 * JH, QA = BM / 16 / WAVES, QB = 2 * HB / 16 / WAVES;
+  static_assert(BM / 16 % WAVES == 0 && 2 * HB / 16 % WAVES == 0 && HB / 16 % QB == 0, "whole chunks, of one half, per wave");
+  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * SLOT];
+  const uint32_t width = PAIR ? HB : 2u * HB;
+  uint32_t tm, tn;
+  gemm_tile_coords((M - 1u) / BM + 1u, (N - 1u) / width + 1u, &tm, &tn, tile);
+  const uint32_t m0 = tm * BM, n0 = tn * width;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t wm = (wave / WGN) * TM, wn = (wave % WGN) * TH;
+  // This lane's place in each chunk that its wave fills: the offset from the
+  // panel's first element of a slice, its first k in the slice, and the end
+  // of k (0: the chunk lies outside the plane).
+  uint32_t offa[QA], ka[QA], enda[QA], offb[QB], kb[QB], endb[QB];
+#pragma unroll
+  for (int q = 0; q < QA; ++q) {
+    const uint32_t slot = (wave * QA + q) * 64u + lane;
+    if constexpr (A_RC) {
+      const uint32_t k = slot / (BM / 8u), m = ((slot % (BM / 8u)) ^ kn_slot_xor<BM>(k)) * 8u;
+      offa[q] = k * M + m;
+      ka[q] = k;
+      enda[q] = m0 + m < M ? K : 0u;
+    } else {
+      const uint32_t r = slot >> 2, c = (slot & 3u) ^ (((r >> 3) & 1u) << 1);
+      offa[q] = r * K + c * 8u;
+      ka[q] = c * 8u;
+      enda[q] = m0 + r < M ? K : 0u;
+    }
+  }
+  const uint32_t half = wave * QB * 16u / HB, nh = PAIR ? n0 : n0 + half * HB;  // the half that this wave fills
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    const uint32_t slot = (wave * QB + q) * 64u + lane - half * (BSL / 8u);
+    if constexpr (B_RC) {
+      const uint32_t k = slot / (HB / 8u), n = ((slot % (HB / 8u)) ^ kn_slot_xor<HB>(k)) * 8u;
+      offb[q] = k * N + n;
+      kb[q] = k;
+      endb[q] = nh + n < N ? K : 0u;
+    } else {
+      const uint32_t r = slot >> 2, c = (slot & 3u) ^ (((r >> 3) & 1u) << 1);
+      offb[q] = r * K + c * 8u;
+      kb[q] = c * 8u;
+      endb[q] = nh + r < N ? K : 0u;
+    }
+  }
+  const uint32_t ns = (K + 31u) / 32u, total = ns * SEGS;
+  uint16_t* ldsp = lds;
+  // Where slice t's panels start; past the last slice every chunk is zeros.
+  struct Slice {
+    const uint16_t *a, *b;
+    uint32_t k0, slot;
+  };
+  auto slice = [&](uint32_t t) {
+    const uint32_t seg = SEGS == 1 || t < ns ? 0u : 1u;
+    Slice s;
+    s.k0 = t < total ? (t - seg * ns) * 32u : K;
+    s.slot = (t & 3u) * SLOT;
+    const uint64_t k = s.k0;
+    s.a = (seg == 0u ? pa0 : pa1) + (A_RC ? k * M + m0 : static_cast<uint64_t>(m0) * K + k);
+    const uint32_t h = PAIR ? half : 0u;
+    const uint16_t* b = h == 0u ? (seg == 0u ? pb00 : pb01) : (seg == 0u ? pb10 : pb11);
+    s.b = b + (B_RC ? k * N + nh : static_cast<uint64_t>(nh) * K + k);
+    return s;
+  };
+  auto load_a = [&](const Slice& s, int q) {
+    const uint16_t* g = s.k0 + ka[q] < enda[q] ? s.a + offa[q] : zero;
+    __builtin_amdgcn_global_load_lds(g, (lds_void*)(ldsp + s.slot + (wave * QA + q) * 512u), 16, 0, 0);
+  };
+  auto load_b = [&](const Slice& s, int q) {
+    const uint16_t* g = s.k0 + kb[q] < endb[q] ? s.b + offb[q] : zero;
+    __builtin_amdgcn_global_load_lds(g, (lds_void*)(ldsp + s.slot + ASL + (wave * QB + q) * 512u), 16, 0, 0);
+  };
+  auto rd_a = [&](uint32_t t, uint32_t i) -> bf16x8 {
+    const uint16_t* As = ldsp + (t & 3u) * SLOT;
+    if constexpr (A_RC) return frag_b16_tr<BM>(As, wm + 16u * i, lane);
+    else return *reinterpret_cast<const bf16x8*>(&As[swz_rows32(wm + 16u * i + (lane & 15u), lane >> 4)]);
+  };
+  auto rd_b = [&](uint32_t t, uint32_t j) -> bf16x8 {  // j < JH: the first half
+    const uint16_t* Bs = ldsp + (t & 3u) * SLOT + ASL + (j / JH) * BSL;
+    const uint32_t n = wn + 16u * (j % JH);
+    if constexpr (B_RC) return frag_b16_tr<HB>(Bs, n, lane);
+    else return *reinterpret_cast<const bf16x8*>(&Bs[swz_rows32(n + (lane & 15u), lane >> 4)]);
+  };
+  f32x4_t acc[IM][JN];
+#pragma unroll
+  for (int i = 0; i < IM; ++i)
+#pragma unroll
+    for (int j = 0; j < JN; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  auto fence = []() { __builtin_amdgcn_sched_barrier(0); };
+  bf16x8 a0[IM], b0[JN], a1[IM], b1[JN];
+  constexpr int LOADS = QA + QB;
+  auto sync = [&]() {  // all but two slices have landed, this wave's LDS reads have completed
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(2 * LOADS, 0));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto step = [&](uint32_t t, const bf16x8* ca, const bf16x8* cb, bf16x8* na, bf16x8* nb) {
+    sync();
+    const Slice s = slice(t + 4u);
+    fence();
+    // MFMA c takes block (i, j), i snaking, so that consecutive ones share an
+    // operand. Operands swapped: a lane ends with four columns of one row.
+#pragma unroll
+    for (int c = 0; c < IM * JN; ++c) {
+      const int j = c / IM, i = (j & 1) ? IM - 1 - c % IM : c % IM;
+      acc[i][j] = mfma_16x16x32_16b<F16>(cb[j], ca[i], acc[i][j]);
+      fence();
+      if (c < IM) na[c] = rd_a(t + 1u, c);
+      else if (c < IM + JN) nb[c - IM] = rd_b(t + 1u, c - IM);
+      constexpr int kFirst = IM * JN - 1 - 2 * LOADS > IM + JN ? IM * JN - 1 - 2 * LOADS : IM * JN - 1 - LOADS;
+      constexpr int kEvery = IM * JN - 1 - 2 * LOADS > IM + JN ? 2 : 1;
+      if (c >= kFirst && (c - kFirst) % kEvery == 0) {
+        const int q = (c - kFirst) / kEvery;
+        if (q < QA) load_a(s, q);
+        else if (q < LOADS) load_b(s, q - QA);
+      }
+      fence();
+    }
+  };
+  if (total > 0u) {
+    for (uint32_t t = 0; t < 4u; ++t) {
+      const Slice s = slice(t);
+#pragma unroll
+      for (int q = 0; q < QA; ++q) load_a(s, q);
+#pragma unroll
+      for (int q = 0; q < QB; ++q) load_b(s, q);
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(3 * LOADS, 0));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < IM; ++i) a0[i] = rd_a(0u, i);
+#pragma unroll
+    for (int j = 0; j < JN; ++j) b0[j] = rd_b(0u, j);
+    for (uint32_t t = 0; t < total; t += 2u) {  // an odd count ends with a slice of zeros
+      step(t, a0, b0, a1, b1);
+      step(t + 1u, a1, b1, a0, b0);
+    }
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));  // no load into LDS is in flight past the loop
+  }
+#pragma unroll
+  for (int i = 0; i < IM; ++i) {
+    const uint32_t m = m0 + wm + 16u * i + (lane & 15u);
+    if (m >= M) continue;
+#pragma unroll
+    for (int j = 0; j < JH; ++j) {
+      const uint32_t n = n0 + wn + 16u * j + 4u * (lane >> 4);
+      if constexpr (PAIR) {
+        if (n < N) epi(m, n, acc[i][j], acc[i][JH + j]);
+      } else {
+        if (n < N) epi(m, n, acc[i][j]);
+        if (n + HB < N) epi(m, n + HB, acc[i][JH + j]);
+      }
+    }
+  }
+}
+
+template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, uint32_t HB, uint32_t WGM, uint32_t WGN, typename Epi>
+__device__ __forceinline__ void product_ring(const Operands<SEGS>& p, const Epi& epi, uint32_t tile) {
+  product_ring_of<F16, A_RC, B_RC, PAIR, SEGS, BM, HB, WGM, WGN>(
+      p.a[0], p.a[SEGS - 1], p.b[0][0], p.b[0][SEGS - 1], p.b[1][0], p.b[1][SEGS - 1],
+      reinterpret_cast<const uint16_t*>(kZeroChunk), p.M, p.N, p.K, epi, tile);
+}
+
 // ------------------------------------------ gradients of the pre-activations
 // One element each: dz = dy act'(z) of a projection, dg = dh u act'(g) and
 // du = dh act(g) of a gated pair. i(e) is (dy, z) or (dh, g, u).

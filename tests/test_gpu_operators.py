@@ -343,6 +343,19 @@ def test_gated_backward_attributes(gpu, M, K, N, elem, attrs):
     check_gated_backward(elem, M, K, N, **attrs)
 
 
+@pytest.mark.parametrize("M,K,N", [(3592, 72, 3608), (3592, 264, 3600)])
+def test_large_planes(gpu, M, K, N):
+    """Planes of many tiles, their last row and column of tiles partial, a
+    reduction that ends inside a slice."""
+    print("large planes", M, K, N, flush=True)
+    check_linear("bf16", M, K, N, act="gelu", bias=True, residual=True)
+    check_gated("f16", M, K, N, save=True)
+    check_linear_backward("bf16", K, M, N, act="gelu", bias=True)  # dw of M x N
+    check_gated_backward("f16", K, M, N)
+    check_linear_backward("f16", M, N, K, bias=True)  # dx of M x N
+    check_gated_backward("bf16", M, N, K)
+
+
 def test_products_empty(gpu):
     """K = 0 leaves the bias and the residual; no tokens, zero weight gradients."""
     check_linear("bf16", 70, 0, 200, bias=True, residual=True)
