@@ -387,8 +387,8 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
     v.push_back(r);
     return v;
   };
-  add("_l", "product_ring<" + targs + ", 256, 128, 2, 4>", 512, 256, 256, with(aligned, When(plane, kLarge, kAll)),
-      "tiles of 256x256, 8 waves, direct to LDS");
+  add("_l", "product_ring<" + targs + ", 256, 128, 2, 2>", 256, 256, 256, with(aligned, When(plane, kLarge, kAll)),
+      "tiles of 256x256, 4 waves of 128x128, direct to LDS");
   add("_s", "product_ring<" + targs + ", 128, 64, 2, 2>", 256, 128, 128, with(aligned, When(plane, 0, kLarge - 1u)),
       "tiles of 128x128, 4 waves, direct to LDS");
   add("", "product_any<" + targs + ">", 256, 128, 128, odd, "tiles of 128x128, any shape and alignment");

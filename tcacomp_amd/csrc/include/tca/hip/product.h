@@ -31,15 +31,33 @@ enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 
 __device__ __forceinline__ float act_sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
 }
-// Phi(z), the normal distribution: erfc keeps its relative precision at -z.
-__device__ __forceinline__ float act_phi(float z) { return 0.5f * erfcf(-0.70710678118654752f * z); }
+// The tail Q(x) = 1 - Phi(x) of the normal distribution over e = exp(-x^2 / 2),
+// x >= 0: t P(t), t = 1 / (1 + 0.36 x), P of degree 6 fitted to erfcx(x /
+// sqrt 2) / 2 over x <= 13.5 by reweighted least squares, 8e-7 off relative to
+// the value. No branches: erfcf has some, and a lane's eight columns wait for each
+// other at them (linear 4096^3 with gelu took 16 us more than without, now 8).
+__device__ __forceinline__ float act_tail(float x) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.36f, x, 1.0f));
+  float p = __builtin_fmaf(0.04734482616186142f, t, -0.18075250089168549f);
+  p = __builtin_fmaf(p, t, 0.1822986900806427f);
+  p = __builtin_fmaf(p, t, 0.02562311850488186f);
+  p = __builtin_fmaf(p, t, 0.14005766808986664f);
+  p = __builtin_fmaf(p, t, 0.14171062409877777f);
+  p = __builtin_fmaf(p, t, 0.1437174379825592f);
+  return p * t;
+}
+// exp(-x^2 / 2); 0 from x = 14 on, where callers hold x.
+__device__ __forceinline__ float act_bell(float x) { return __builtin_amdgcn_exp2f(-0.72134752044448170f * x * x); }
+__device__ __forceinline__ float act_far(float z) { return __builtin_fminf(__builtin_fabsf(z), 14.0f); }
 
 template <int ACT>
 __device__ __forceinline__ float act(float z) {
   if constexpr (ACT == kActRelu) return z < 0.0f ? 0.0f : z;
   else if constexpr (ACT == kActSilu) return z * act_sigmoid(z);
-  else if constexpr (ACT == kActGelu) return z * act_phi(z);
-  else if constexpr (ACT == kActGeluTanh)  // 1 + tanh(u) = 2 sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3)
+  else if constexpr (ACT == kActGelu) {  // z Phi(z) = max(z, 0) - |z| Q(|z|)
+    const float x = act_far(z);
+    return (z < 0.0f ? 0.0f : z) - x * (act_tail(x) * act_bell(x));
+  } else if constexpr (ACT == kActGeluTanh)  // 1 + tanh(u) = 2 sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3)
     return z * act_sigmoid(1.59576912160573071f * z * __builtin_fmaf(0.044715f * z, z, 1.0f));
   else return z;
 }
@@ -51,7 +69,9 @@ __device__ __forceinline__ float act_slope(float z) {
     const float s = act_sigmoid(z);
     return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
   } else if constexpr (ACT == kActGelu) {
-    return act_phi(z) + z * (0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z));
+    const float x = act_far(z), e = act_bell(x), q = act_tail(x) * e;
+    const float d = 0.39894228040143268f * (x * e);  // |z| phi(z)
+    return z < 0.0f ? q - d : z == z ? (1.0f - q) + d : z;
   } else if constexpr (ACT == kActGeluTanh) {
     const float s = act_sigmoid(1.59576912160573071f * z * __builtin_fmaf(0.044715f * z, z, 1.0f));
     const float du = 1.59576912160573071f * __builtin_fmaf(3.0f * 0.044715f * z, z, 1.0f);
@@ -62,34 +82,10 @@ __device__ __forceinline__ float act_slope(float z) {
 }
 
 // ------------------------------------------------------------- epilogues
-// Each takes four consecutive columns n .. n + 3 of row m < M, n < N, and
-// stores those before N.
-template <typename T>
-__device__ __forceinline__ f32x4_t load4(const T* p, uint32_t n, uint32_t N) {
-  f32x4_t f;
-  if (n + 4u <= N) {
-    const vec<T, 4> v = load_vec_any<T, 4, false>(p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = static_cast<float>(v[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = n + e < N ? static_cast<float>(p[e]) : 0.0f;
-  }
-  return f;
-}
-template <typename T>
-__device__ __forceinline__ void store4(T* p, uint32_t n, uint32_t N, f32x4_t f) {
-  if (n + 4u <= N) {
-    vec<T, 4> v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v.set(e, static_cast<T>(f[e]));
-    store_vec_any<T, 4, false>(p, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < N) p[e] = static_cast<T>(f[e]);
-  }
-}
+// Each takes eight consecutive columns n .. n + 7 of row m < M, n < N, and
+// stores those before N (WHOLE: all of them); fetch() loads what it reads of
+// memory, ahead of the call.
+struct NoFetch {};
 
 // y = res + act(z), z = v + b [z stored too]. res may be y: an element is
 // read by the lane that then writes it.
@@ -100,14 +96,29 @@ struct LinearStore {
   T* y;
   T* z;
   uint32_t N;
-  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, f32x4_t v) const {
-    const uint64_t at = static_cast<uint64_t>(m) * N + n;
-    if constexpr (BIAS) v += load4(b + n, n, N);
-    if constexpr (SAVE) store4(z + at, n, N, v);
+  struct Fetch {
+    vec<T, 8> res, b;
+  };
+  template <bool WHOLE>
+  __device__ __forceinline__ Fetch fetch(uint32_t m, uint32_t n) const {
+    Fetch f;
+    if constexpr (RES) f.res = row_raw<8, WHOLE>(res + static_cast<uint64_t>(m) * N, n, N);
+    if constexpr (BIAS) f.b = row_raw<8, WHOLE>(b, n, N);
+    return f;
+  }
+  template <bool WHOLE>
+  __device__ __forceinline__ void store(uint32_t m, uint32_t n, const Fetch& f, float (&v)[8]) const {
+    const uint64_t row = static_cast<uint64_t>(m) * N;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = act<ACT>(v[e]);
-    if constexpr (RES) v += load4(res + at, n, N);
-    store4(y + at, n, N, v);
+    for (int e = 0; e < 8; ++e)
+      if constexpr (BIAS) v[e] += static_cast<float>(f.b[e]);
+    if constexpr (SAVE) row_store<8, WHOLE>(z + row, n, N, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = act<ACT>(v[e]);
+      if constexpr (RES) v[e] += static_cast<float>(f.res[e]);
+    }
+    row_store<8, WHOLE>(y + row, n, N, v);
   }
 };
 // h = act(g) u, g = v0 + bg, u = v1 + bu [g and u stored too].
@@ -119,19 +130,34 @@ struct GatedStore {
   T* g;
   T* u;
   uint32_t N;
-  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, f32x4_t v0, f32x4_t v1) const {
-    const uint64_t at = static_cast<uint64_t>(m) * N + n;
+  struct Fetch {
+    vec<T, 8> bg, bu;
+  };
+  template <bool WHOLE>
+  __device__ __forceinline__ Fetch fetch(uint32_t, uint32_t n) const {
+    Fetch f;
     if constexpr (BIAS) {
-      v0 += load4(bg + n, n, N);
-      v1 += load4(bu + n, n, N);
+      f.bg = row_raw<8, WHOLE>(bg, n, N);
+      f.bu = row_raw<8, WHOLE>(bu, n, N);
     }
+    return f;
+  }
+  template <bool WHOLE>
+  __device__ __forceinline__ void store(uint32_t m, uint32_t n, const Fetch& f, float (&v0)[8], float (&v1)[8]) const {
+    const uint64_t row = static_cast<uint64_t>(m) * N;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if constexpr (BIAS) {
+        v0[e] += static_cast<float>(f.bg[e]);
+        v1[e] += static_cast<float>(f.bu[e]);
+      }
     if constexpr (SAVE) {
-      store4(g + at, n, N, v0);
-      store4(u + at, n, N, v1);
+      row_store<8, WHOLE>(g + row, n, N, v0);
+      row_store<8, WHOLE>(u + row, n, N, v1);
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v0[e] = act<ACT>(v0[e]) * v1[e];
-    store4(h + at, n, N, v0);
+    for (int e = 0; e < 8; ++e) v0[e] = act<ACT>(v0[e]) * v1[e];
+    row_store<8, WHOLE>(h + row, n, N, v0);
   }
 };
 // The results themselves: of one product, or of a pair.
@@ -140,14 +166,95 @@ struct PlainStore {
   T* c;
   T* c1;
   uint32_t N;
-  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, f32x4_t v) const {
-    store4(c + static_cast<uint64_t>(m) * N + n, n, N, v);
+  using Fetch = NoFetch;
+  template <bool WHOLE>
+  __device__ __forceinline__ Fetch fetch(uint32_t, uint32_t) const {
+    return {};
   }
-  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, f32x4_t v0, f32x4_t v1) const {
-    store4(c + static_cast<uint64_t>(m) * N + n, n, N, v0);
-    store4(c1 + static_cast<uint64_t>(m) * N + n, n, N, v1);
+  template <bool WHOLE>
+  __device__ __forceinline__ void store(uint32_t m, uint32_t n, const Fetch&, float (&v)[8]) const {
+    row_store<8, WHOLE>(c + static_cast<uint64_t>(m) * N, n, N, v);
+  }
+  template <bool WHOLE>
+  __device__ __forceinline__ void store(uint32_t m, uint32_t n, const Fetch&, float (&v0)[8], float (&v1)[8]) const {
+    row_store<8, WHOLE>(c + static_cast<uint64_t>(m) * N, n, N, v0);
+    row_store<8, WHOLE>(c1 + static_cast<uint64_t>(m) * N, n, N, v1);
   }
 };
+
+// A wave's results to the epilogue: IM blocks of 16 rows by JH blocks of 16
+// columns of either half (acc[i][j], j < JH the first half), 64 rows at a time
+// through `lds` (64 x 32 JH floats of the wave's own), so that a lane takes
+// eight consecutive columns, the memory accesses of a row are whole lines, and
+// the epilogue's code is there once and not once for each block. 16-byte slot
+// c of row r lies at c ^ (r % 16): the writes of a block's 16 rows cover the
+// banks once. Four chunks a turn, the next turn's loads issued before this
+// one's stores: a wave has its SIMD to itself, nothing else covers their
+// latency. WHOLE: every chunk lies inside the plane.
+template <int IM, int JH, bool PAIR, bool WHOLE, typename Epi>
+__device__ __forceinline__ void product_store(const f32x4_t (&acc)[IM][2 * JH], float* lds, uint32_t m0, uint32_t n0,
+                                              uint32_t half, uint32_t M, uint32_t N, const Epi& epi, uint32_t lane) {
+  constexpr uint32_t TH = 16u * JH, PITCH = 2u * TH, CHUNKS = PAIR ? TH / 8u : TH / 4u;  // of a row
+  constexpr uint32_t TURN = 4, TURNS = CHUNKS / TURN, PASSES = IM / 4;
+  static_assert(IM % 4 == 0 && CHUNKS % TURN == 0, "64 rows at a time, whole turns");
+  typename Epi::Fetch now[TURN], next[TURN];
+  auto row_of = [&](uint32_t t) { return (t * 64u + lane) / CHUNKS; };  // of a pass
+  auto col_of = [&](uint32_t t) { return (t * 64u + lane) % CHUNKS; };
+  auto fetch = [&](uint32_t turn, typename Epi::Fetch (&f)[TURN]) {  // turns counted over the passes
+#pragma unroll
+    for (uint32_t i = 0; i < TURN; ++i) {
+      const uint32_t t = turn % TURNS * TURN + i, k = col_of(t);
+      const uint32_t m = m0 + 64u * (turn / TURNS) + row_of(t), n = n0 + k / (TH / 8u) * half + k % (TH / 8u) * 8u;
+      if (WHOLE || (m < M && n < N)) f[i] = epi.template fetch<WHOLE>(m, n);
+    }
+  };
+  fetch(0u, now);
+#pragma unroll 1
+  for (uint32_t pass = 0; pass < PASSES; ++pass) {
+    wave_exchange();
+#pragma unroll
+    for (int p = 0; p < static_cast<int>(PASSES); ++p) {
+      if (pass != static_cast<uint32_t>(p)) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2 * JH; ++j) {
+          const uint32_t r = 16u * i + (lane & 15u), c = 4u * j + (lane >> 4);
+          *reinterpret_cast<f32x4_t*>(&lds[r * PITCH + ((c ^ (r & 15u)) << 2)]) = acc[4 * p + i][j];
+        }
+    }
+    wave_exchange();
+#pragma unroll 1
+    for (uint32_t b = 0; b < TURNS; ++b) {
+      const uint32_t turn = pass * TURNS + b;
+      if (turn + 1u < PASSES * TURNS) fetch(turn + 1u, next);
+#pragma unroll
+      for (uint32_t i = 0; i < TURN; ++i) {
+        const uint32_t t = b * TURN + i, r = row_of(t), k = col_of(t), h = k / (TH / 8u), c = h * (TH / 4u) + k % (TH / 8u) * 2u;
+        const uint32_t m = m0 + 64u * pass + r, n = n0 + h * half + k % (TH / 8u) * 8u;
+        const float* row = &lds[r * PITCH];
+        auto take = [&](uint32_t s, float (&v)[8]) {
+          const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(&row[(s ^ (r & 15u)) << 2]);
+          const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(&row[((s + 1u) ^ (r & 15u)) << 2]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = lo[e];
+            v[4 + e] = hi[e];
+          }
+        };
+        float v0[8], v1[8];
+        take(c, v0);
+        if constexpr (PAIR) take(c + TH / 4u, v1);
+        if (WHOLE || (m < M && n < N)) {
+          if constexpr (PAIR) epi.template store<WHOLE>(m, n, now[i], v0, v1);
+          else epi.template store<WHOLE>(m, n, now[i], v0);
+        }
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < TURN; ++i) now[i] = next[i];
+    }
+  }
+}
 
 // ------------------------------------------------------------- operands
 // M x N results over SEGS segments of K. a[s]: [M][K] or, A_RC, [K][M]; b[h][s]
@@ -263,13 +370,11 @@ __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& 
       }
     }
   };
-  f32x4_t acc[2][4][2];
+  f32x4_t acc[4][4];  // [block of rows][2 h + block of columns]
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[h][i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   auto compute = [&](uint32_t t) {
     const uint16_t* As = lds + (t & 1u) * BUF;
 #pragma unroll
@@ -290,7 +395,7 @@ __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& 
           else fb = *reinterpret_cast<const bf16x8*>(&Bs[swz_rows64(wn + 16u * j + (lane & 15u), 4u * s + (lane >> 4))]);
           // Operands swapped: a lane ends with four consecutive columns of one row.
 #pragma unroll
-          for (uint32_t i = 0; i < 4u; ++i) acc[h][i][j] = mfma_16x16x32_16b<F16>(fb, fa[i], acc[h][i][j]);
+          for (uint32_t i = 0; i < 4u; ++i) acc[i][2u * h + j] = mfma_16x16x32_16b<F16>(fb, fa[i], acc[i][2u * h + j]);
         }
       }
     }
@@ -306,27 +411,18 @@ __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& 
       __syncthreads();
     }
   }
-#pragma unroll
-  for (uint32_t i = 0; i < 4u; ++i) {
-    const uint32_t m = m0 + wm + 16u * i + (lane & 15u);
-    if (m >= M) continue;
-#pragma unroll
-    for (uint32_t j = 0; j < 2u; ++j) {
-      const uint32_t n = n0 + wn + 16u * j + 4u * (lane >> 4);
-      if constexpr (PAIR) {
-        if (n < N) epi(m, n, acc[0][i][j], acc[1][i][j]);
-      } else {
-        if (n < N) epi(m, n, acc[0][i][j]);
-        if (n + HB < N) epi(m, n + HB, acc[1][i][j]);
-      }
-    }
-  }
+  // (the last slice's barrier: no wave reads the slices any more)
+  product_store<4, 2, PAIR, false>(acc, reinterpret_cast<float*>(lds) + wave * (64u * 64u), m0 + wm, n0 + wn, HB, M, N, epi, lane);
 }
 
 // ------------------------- rows of whole 16-byte chunks: straight into LDS
 // What chunks that lie outside an operand read (a static constant of the code
 // object): rows past the end and slices past the last add zeros to the sums.
 static __device__ __attribute__((aligned(16))) const uint32_t kZeroChunk[4] = {0u, 0u, 0u, 0u};
+
+// Extents up to here keep a lane's offset in a panel (256 rows of K, or 32
+// rows of M or N, in bytes) within 32 bits.
+constexpr uint32_t kInnerMost = 1u << 22;
 
 // A tile of BM x 2 HB (a pair: BM x HB of each product), WGM x WGN waves, each
 // (BM / WGM) rows by HB / WGN columns of either half, for operands whose rows
@@ -398,6 +494,11 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
   }
   const uint32_t ns = (K + 31u) / 32u, total = ns * SEGS;
   uint16_t* ldsp = lds;
+  // Slices whose chunks all lie inside the operands, for a tile that does:
+  // their loads take the panel's address from scalar registers and a 32-bit
+  // offset a lane, with no test (which costs a tenth of the whole time).
+  const bool inner = m0 + BM <= M && n0 + width <= N && M <= kInnerMost && N <= kInnerMost && K <= kInnerMost;
+  const uint32_t whole = !inner ? 0u : K % 32u == 0u ? total : SEGS == 1 ? K / 32u : 0u;
   // Where slice t's panels start; past the last slice every chunk is zeros.
   struct Slice {
     const uint16_t *a, *b;
@@ -415,12 +516,16 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
     s.b = b + (B_RC ? k * N + nh : static_cast<uint64_t>(nh) * K + k);
     return s;
   };
-  auto load_a = [&](const Slice& s, int q) {
-    const uint16_t* g = s.k0 + ka[q] < enda[q] ? s.a + offa[q] : zero;
+  auto load_a = [&](auto fast, const Slice& s, int q) {
+    const uint16_t* g = s.a + offa[q];
+    if constexpr (decltype(fast)::value) g = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(s.a) + 2u * offa[q]);
+    else g = s.k0 + ka[q] < enda[q] ? g : zero;
     __builtin_amdgcn_global_load_lds(g, (lds_void*)(ldsp + s.slot + (wave * QA + q) * 512u), 16, 0, 0);
   };
-  auto load_b = [&](const Slice& s, int q) {
-    const uint16_t* g = s.k0 + kb[q] < endb[q] ? s.b + offb[q] : zero;
+  auto load_b = [&](auto fast, const Slice& s, int q) {
+    const uint16_t* g = s.b + offb[q];
+    if constexpr (decltype(fast)::value) g = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(s.b) + 2u * offb[q]);
+    else g = s.k0 + kb[q] < endb[q] ? g : zero;
     __builtin_amdgcn_global_load_lds(g, (lds_void*)(ldsp + s.slot + ASL + (wave * QB + q) * 512u), 16, 0, 0);
   };
   auto rd_a = [&](uint32_t t, uint32_t i) -> bf16x8 {
@@ -440,6 +545,20 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
 #pragma unroll
     for (int j = 0; j < JN; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   auto fence = []() { __builtin_amdgcn_sched_barrier(0); };
+  // 64 blocks a wave: the accumulators are tied to AGPRs by inline-asm MFMAs,
+  // with the hazards covered as at gemm_bf16_4w (the operands are results of
+  // LDS reads only; wait states before the first and after the last).
+  constexpr bool kAgpr = IM * JN >= 64;
+  if constexpr (kAgpr) {
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+#pragma unroll
+      for (int j = 0; j < JN; ++j) asm volatile("" : "+a"(acc[i][j]));
+    asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
+    fence();
+  }
+  using Fast = std::true_type;
+  using Checked = std::false_type;
   bf16x8 a0[IM], b0[JN], a1[IM], b1[JN];
   constexpr int LOADS = QA + QB;
   auto sync = [&]() {  // all but two slices have landed, this wave's LDS reads have completed
@@ -448,7 +567,7 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  auto step = [&](uint32_t t, const bf16x8* ca, const bf16x8* cb, bf16x8* na, bf16x8* nb) {
+  auto step = [&](auto fast, uint32_t t, const bf16x8* ca, const bf16x8* cb, bf16x8* na, bf16x8* nb) {
     sync();
     const Slice s = slice(t + 4u);
     fence();
@@ -457,57 +576,61 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
 #pragma unroll
     for (int c = 0; c < IM * JN; ++c) {
       const int j = c / IM, i = (j & 1) ? IM - 1 - c % IM : c % IM;
-      acc[i][j] = mfma_16x16x32_16b<F16>(cb[j], ca[i], acc[i][j]);
+      if constexpr (kAgpr) mfma16_bf16_acc<F16>(acc[i][j], cb[j], ca[i]);
+      else acc[i][j] = mfma_16x16x32_16b<F16>(cb[j], ca[i], acc[i][j]);
       fence();
-      if (c < IM) na[c] = rd_a(t + 1u, c);
-      else if (c < IM + JN) nb[c - IM] = rd_b(t + 1u, c - IM);
-      constexpr int kFirst = IM * JN - 1 - 2 * LOADS > IM + JN ? IM * JN - 1 - 2 * LOADS : IM * JN - 1 - LOADS;
-      constexpr int kEvery = IM * JN - 1 - 2 * LOADS > IM + JN ? 2 : 1;
-      if (c >= kFirst && (c - kFirst) % kEvery == 0) {
-        const int q = (c - kFirst) / kEvery;
-        if (q < QA) load_a(s, q);
-        else if (q < LOADS) load_b(s, q - QA);
+      // The reads of the next fragments, then the loads, evenly over the MFMAs
+      // but the last few: in a burst, four SIMDs ask for twice what LDS gives.
+      constexpr int kOps = IM + JN + LOADS, kOver = IM * JN - 4;
+      for (int o = c * kOps / kOver; o < (c + 1) * kOps / kOver && o < kOps; ++o) {
+        if (o < IM) na[o] = rd_a(t + 1u, o);
+        else if (o < IM + JN) nb[o - IM] = rd_b(t + 1u, o - IM);
+        else if (o < IM + JN + QA) load_a(fast, s, o - IM - JN);
+        else load_b(fast, s, o - IM - JN - QA);
       }
       fence();
     }
   };
-  if (total > 0u) {
-    for (uint32_t t = 0; t < 4u; ++t) {
-      const Slice s = slice(t);
+  for (uint32_t t = 0; t < 4u; ++t) {
+    const Slice s = slice(t);
 #pragma unroll
-      for (int q = 0; q < QA; ++q) load_a(s, q);
+    for (int q = 0; q < QA; ++q) load_a(Checked{}, s, q);
 #pragma unroll
-      for (int q = 0; q < QB; ++q) load_b(s, q);
-    }
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(waitcnt_imm(3 * LOADS, 0));
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < IM; ++i) a0[i] = rd_a(0u, i);
-#pragma unroll
-    for (int j = 0; j < JN; ++j) b0[j] = rd_b(0u, j);
-    for (uint32_t t = 0; t < total; t += 2u) {  // an odd count ends with a slice of zeros
-      step(t, a0, b0, a1, b1);
-      step(t + 1u, a1, b1, a0, b0);
-    }
-    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));  // no load into LDS is in flight past the loop
+    for (int q = 0; q < QB; ++q) load_b(Checked{}, s, q);
   }
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(waitcnt_imm(3 * LOADS, 0));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < IM; ++i) {
-    const uint32_t m = m0 + wm + 16u * i + (lane & 15u);
-    if (m >= M) continue;
+  for (int i = 0; i < IM; ++i) a0[i] = rd_a(0u, i);
 #pragma unroll
-    for (int j = 0; j < JH; ++j) {
-      const uint32_t n = n0 + wn + 16u * j + 4u * (lane >> 4);
-      if constexpr (PAIR) {
-        if (n < N) epi(m, n, acc[i][j], acc[i][JH + j]);
-      } else {
-        if (n < N) epi(m, n, acc[i][j]);
-        if (n + HB < N) epi(m, n + HB, acc[i][JH + j]);
-      }
-    }
+  for (int j = 0; j < JN; ++j) b0[j] = rd_b(0u, j);
+  // An odd count ends with a slice of zeros; K = 0 is two of them (a branch
+  // round the loop would hold the accumulators in two places, and spill).
+  uint32_t t = 0u;
+  for (; t + 5u < whole; t += 2u) {
+    step(Fast{}, t, a0, b0, a1, b1);
+    step(Fast{}, t + 1u, a1, b1, a0, b0);
   }
+  do {
+    step(Checked{}, t, a0, b0, a1, b1);
+    step(Checked{}, t + 1u, a1, b1, a0, b0);
+    t += 2u;
+  } while (t < total);
+  // No load into LDS is in flight past the loop, in any wave.
+  __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if constexpr (kAgpr) {
+    fence();
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+    fence();
+  }
+  static_assert(WAVES * 64u * 2u * TH * 4u <= sizeof(lds), "64 rows of every wave");
+  float* own = reinterpret_cast<float*>(lds) + wave * (64u * 2u * TH);
+  if (m0 + BM <= M && n0 + width <= N) product_store<IM, JH, PAIR, true>(acc, own, m0 + wm, n0 + wn, HB, M, N, epi, lane);
+  else product_store<IM, JH, PAIR, false>(acc, own, m0 + wm, n0 + wn, HB, M, N, epi, lane);
 }
 
 template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, uint32_t HB, uint32_t WGM, uint32_t WGN, typename Epi>

@@ -11,10 +11,11 @@ namespace hip {
 template <typename T>
 constexpr int kRowE = 16 / static_cast<int>(sizeof(T));  // values per 16-byte vector
 
-// E values of a row from column c on, as f32; zeros past the end.
-template <int E, typename T>
+// E values of a row from column c on, as f32; zeros past the end. WHOLE: all
+// of them lie before it.
+template <int E, bool WHOLE = false, typename T>
 __device__ __forceinline__ void row_load(const T* row, uint32_t c, uint32_t C, float (&f)[E]) {
-  if (c < C && C - c >= static_cast<uint32_t>(E)) {
+  if (WHOLE || (c < C && C - c >= static_cast<uint32_t>(E))) {
     const vec<T, E> v = load_vec_any<T, E, false>(row + c);
 #pragma unroll
     for (int e = 0; e < E; ++e) f[e] = static_cast<float>(v[e]);
@@ -24,9 +25,9 @@ __device__ __forceinline__ void row_load(const T* row, uint32_t c, uint32_t C, f
   }
 }
 // ... and back, rounded to nearest once.
-template <int E, typename T>
+template <int E, bool WHOLE = false, typename T>
 __device__ __forceinline__ void row_store(T* row, uint32_t c, uint32_t C, const float (&f)[E]) {
-  if (c < C && C - c >= static_cast<uint32_t>(E)) {
+  if (WHOLE || (c < C && C - c >= static_cast<uint32_t>(E))) {
     vec<T, E> v;
 #pragma unroll
     for (int e = 0; e < E; ++e) v.set(e, static_cast<T>(f[e]));
@@ -36,6 +37,16 @@ __device__ __forceinline__ void row_store(T* row, uint32_t c, uint32_t C, const 
     for (int e = 0; e < E; ++e)
       if (c + e < C) row[c + e] = static_cast<T>(f[e]);
   }
+}
+
+// The same values as they lie in memory, for loads ahead of their use.
+template <int E, bool WHOLE = false, typename T>
+__device__ __forceinline__ vec<T, E> row_raw(const T* row, uint32_t c, uint32_t C) {
+  if (WHOLE || (c < C && C - c >= static_cast<uint32_t>(E))) return load_vec_any<T, E, false>(row + c);
+  vec<T, E> v;
+#pragma unroll
+  for (int e = 0; e < E; ++e) v.set(e, c + e < C ? row[c + e] : static_cast<T>(0.0f));
+  return v;
 }
 
 // Partial rows of a sum over R rows: one for each `rows` of them, at most
