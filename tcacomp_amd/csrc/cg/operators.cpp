@@ -139,7 +139,12 @@ class Writer {
     std::string suffix, params, body, grid, detail;  // params: tensor, dim and scalar names; grid: terms
     uint32_t block = 256;
     std::vector<std::string> records;  // when, unless, split
-    std::string attribute;             // of the function
+    // Functions that stand in for it: their suffix, body and what they are, and
+    // the plan's bounds (after "form <symbol>"); one may be listed again with others.
+    struct Form {
+      std::string suffix, body, detail, bounds;
+    };
+    std::vector<Form> forms;
   };
   void Add(const Kernel& k) {
     const std::string symbol = "tca_" + program_ + k.suffix;
@@ -159,13 +164,19 @@ class Writer {
         args += "arg dim " + p + "\n";
       }
     }
-    body_ << "// " << k.detail << "\nextern \"C\" __global__ void __launch_bounds__(" << k.block << ") "
-          << (k.attribute.empty() ? "" : k.attribute + " ") << symbol << "(" << sig << ") {\n"
-          << k.body << "}\n\n";
+    auto function = [&](const std::string& name, const std::string& detail, const std::string& body) {
+      body_ << "// " << detail << "\nextern \"C\" __global__ void __launch_bounds__(" << k.block << ") " << name << "("
+            << sig << ") {\n" << body << "}\n\n";
+    };
+    function(symbol, k.detail, k.body);
+    std::set<std::string> written;
+    for (const auto& f : k.forms)
+      if (written.insert(f.suffix).second) function("tca_" + program_ + f.suffix, f.detail, f.body);
     int terms = 0;
     std::istringstream g(k.grid);
     for (std::string t; g >> t;) ++terms;
     kernels_ << "kernel " << symbol << " " << k.block << " 0 " << terms << " " << k.grid << "\n" << args;
+    for (const auto& f : k.forms) kernels_ << "form tca_" << program_ << f.suffix << " " << f.bounds << "\n";
     for (const auto& r : k.records) kernels_ << r << "\n";
     report_ << symbol << " operator chains= " << k.detail << "\n";
     KernelInfo info;
@@ -359,39 +370,48 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   }
   ops << "  p.M = " << p.M << ";\n  p.N = " << p.N << ";\n  p.K = " << p.K << ";\n  const auto epi = " << p.epi << ";\n";
   const std::string f16 = Bool(a.elem == "f16");
-  auto add = [&](const std::string& suffix, const std::string& call, uint32_t block, uint32_t rows, uint32_t cols,
-                 const std::vector<std::string>& records, const std::string& detail) {
-    Writer::Kernel k;
-    k.suffix = p.suffix + suffix;
-    k.params = p.params;
-    k.block = block;
-    k.body = ops.str() + "  tca::hip::" + call + "(p, epi, blockIdx.x);\n";
-    k.grid = p.M + "/" + std::to_string(rows) + " " + p.N + "/" + std::to_string(p.pair ? cols / 2u : cols);
-    k.records = records;
-    k.detail = p.what + ", " + detail;
-    w->Add(k);
-  };
   const std::string targs = f16 + ", " + Bool(p.a_rc) + ", " + Bool(p.b_rc) + ", " + Bool(p.pair) + ", " + std::to_string(p.segs);
+  auto body = [&](const std::string& call) { return ops.str() + "  tca::hip::" + call + "(p, epi, blockIdx.x);\n"; };
+  auto tiles = [&](uint32_t rows, uint32_t cols) {
+    return p.M + "/" + std::to_string(rows) + " " + p.N + "/" + std::to_string(p.pair ? cols / 2u : cols);
+  };
   // Rows of whole 16-byte chunks, of both operands, go straight into LDS.
-  std::vector<std::string> whole;
-  for (const std::string& d : {p.a_rc ? p.M : p.K, p.b_rc ? p.N : p.K})
-    if (whole.empty() || whole[0] != d) whole.push_back(d);
   std::vector<std::string> aligned, odd;
-  for (const auto& d : whole) {
+  for (const std::string& d : std::set<std::string>{p.a_rc ? p.M : p.K, p.b_rc ? p.N : p.K}) {
     aligned.push_back(When(d, 0, kMost, 8));
     odd.push_back("unless " + d + " 0 " + std::to_string(kMost) + " 8 0");
   }
-  const std::string plane = p.M + "*" + p.N;
-  const uint64_t kLarge = (p.pair ? 32768ull : 65536ull) * 192u, kAll = 18446744073709551615ull;
-  auto with = [](std::vector<std::string> v, const std::string& r) {
-    v.push_back(r);
-    return v;
+  Writer::Kernel k;
+  k.suffix = p.suffix + "_r";
+  k.params = p.params;
+  k.records = aligned;
+  k.body = body("product_ring<" + targs + ", 128, 64, 2, 2, 5, 5>");
+  k.grid = tiles(128, 128);
+  k.detail = p.what + ", tiles of 128x128 (256x256, 256x128 where they fill the card), 4 waves, direct to LDS";
+  auto form = [&](const char* suffix, const std::string& what, const std::string& config, uint32_t rows, uint32_t cols,
+                  uint32_t most, const std::string& of) {
+    const std::string grid = tiles(rows, cols);
+    // its grid, then the bound: at least `most` tiles, of `of`
+    k.forms.push_back({p.suffix + suffix, body("product_ring<" + targs + ", " + config + ">"), p.what + ", " + what,
+                       "0 2 1 2 " + grid + " " + std::to_string(most) + " 2 " + of});
   };
-  add("_l", "product_ring<" + targs + ", 256, 128, 2, 2>", 256, 256, 256, with(aligned, When(plane, kLarge, kAll)),
-      "tiles of 256x256, 4 waves of 128x128, direct to LDS");
-  add("_s", "product_ring<" + targs + ", 128, 64, 2, 2>", 256, 128, 128, with(aligned, When(plane, 0, kLarge - 1u)),
-      "tiles of 128x128, 4 waves, direct to LDS");
-  add("", "product_any<" + targs + ">", 256, 128, 128, odd, "tiles of 128x128, any shape and alignment");
+  const std::string large = tiles(256, 256), tall = tiles(256, 128), small = tiles(128, 128);
+  const std::string what_l = "tiles of 256x256", what_m = "tiles of 256x128", what_s = "tiles of 128x128, two workgroups a CU";
+  const std::string cfg_l = "256, 128, 2, 2, 3, 2", cfg_m = "256, 64, 2, 2, 3, 3", cfg_s = "128, 64, 2, 2, 3, 2";
+  form("_l", what_l, cfg_l, 256, 256, 385, large);
+  form("_m", what_m, cfg_m, 256, 128, 257, large);
+  form("_l", what_l, cfg_l, 256, 256, 192, large);
+  form("_m", what_m, cfg_m, 256, 128, 192, tall);
+  form("_s", what_s, cfg_s, 128, 128, 257, small);
+  w->Add(k);
+  Writer::Kernel any;
+  any.suffix = p.suffix;
+  any.params = p.params;
+  any.records = odd;
+  any.body = body("product_any<" + targs + ">");
+  any.grid = tiles(128, 128);
+  any.detail = p.what + ", tiles of 128x128, any shape and alignment";
+  w->Add(any);
 }
 
 void EmitForward(const Attrs& a, bool gated, Writer* w) {

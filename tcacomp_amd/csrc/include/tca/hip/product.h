@@ -420,124 +420,159 @@ __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& 
 // object): rows past the end and slices past the last add zeros to the sums.
 static __device__ __attribute__((aligned(16))) const uint32_t kZeroChunk[4] = {0u, 0u, 0u, 0u};
 
-// Extents up to here keep a lane's offset in a panel (256 rows of K, or 32
+// Extents up to here keep a lane's offset in a panel (256 rows of K, or 64
 // rows of M or N, in bytes) within 32 bits.
 constexpr uint32_t kInnerMost = 1u << 22;
+
+// How a lane reads the MFMA operands of a 64-deep panel of W rows
+// (K-contiguous) or W columns (RC), `blocks` of 16 from `first` on: for k 32 h ..
+// 32 h + 31 of block i, a byte offset in the panel, of which only few depend on
+// the lane (one for each h, or for each block), the rest being constants of
+// the instruction. (RC: ds_read_b64_tr_b16 as at frag_b16_tr; the swizzle of row
+// k leaves out bits 2, 4 and 5 of k.)
+template <bool RC, uint32_t W, int BLOCKS>
+struct Frags {
+  uint32_t off[RC ? BLOCKS : 2];
+  __device__ __forceinline__ Frags(uint32_t first, uint32_t lane) {
+    const uint32_t g = lane >> 4, j = lane & 15u;
+    if constexpr (RC) {
+#pragma unroll
+      for (int i = 0; i < BLOCKS; ++i) off[i] = 2u * swz_kn<W>(8u * g + (j >> 2), first + 16u * i + 4u * (j & 3u));
+    } else {
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) off[h] = 2u * swz_rows64(first + j, 4u * h + g);
+    }
+  }
+  // `panel`: bytes from `lds`, a scalar.
+  __device__ __forceinline__ bf16x8 read(const uint16_t* lds, uint32_t panel, int h, int i) const {
+    if constexpr (RC) {
+      const char* p = reinterpret_cast<const char*>(lds) + (panel + off[i]) + 64 * static_cast<int>(W) * h;
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p + 8 * static_cast<int>(W)));
+      typedef short i16x8 __attribute__((ext_vector_type(8)));
+      const i16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      return __builtin_bit_cast(bf16x8, v);
+    } else {
+      return *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(lds) + (panel + off[h]) + 2048 * i);
+    }
+  }
+};
+
+// How the lanes of WAVES waves fill a 64-deep panel of W rows (K-contiguous)
+// or W columns (RC): chunk q of a wave is chunk q WAVES + wave of the panel, so
+// that a lane's places in them differ by a multiple of the pitch, a scalar
+// (and, for 256 columns, by a swizzle that alternates with q).
+template <bool RC, uint32_t W, uint32_t WAVES>
+struct Fill {
+  static constexpr uint32_t kRows = RC ? 512u / W : 8u;  // rows of memory in a chunk
+  static constexpr bool kTwo = RC && WAVES * kRows == 8u;
+  static_assert(!RC || WAVES * kRows % 8u == 0u, "the swizzle of row k alternates with q at most");
+  uint32_t off[kTwo ? 2 : 1], row, col[kTwo ? 2 : 1];  // elements from the panel's first, row and column in it
+  __device__ __forceinline__ Fill(uint32_t wave, uint32_t lane, uint32_t pitch) {
+    row = wave * kRows + lane / (RC ? W / 8u : 8u);
+#pragma unroll
+    for (uint32_t i = 0; i < (kTwo ? 2u : 1u); ++i) {
+      if constexpr (RC) col[i] = ((lane % (W / 8u)) ^ kn_slot_xor<W>(row + 8u * i)) * 8u;
+      else col[i] = ((lane & 7u) ^ (row & 6u)) * 8u;  // the inverse of swz_rows64
+      off[i] = row * pitch + col[i];
+    }
+  }
+  // Chunk q of the panel at p, its first element (k0, c0) in k and its own
+  // index, K and C their ends.
+  template <bool FAST>
+  __device__ __forceinline__ void load(const uint16_t* p, const uint16_t* zero, uint16_t* lds, int q, uint32_t pitch, uint32_t wave,
+                                       uint32_t k0, uint32_t c0, uint32_t K, uint32_t C) const {
+    constexpr uint32_t kStep = WAVES * kRows;
+    const uint32_t i = kTwo ? q & 1 : 0u, k = RC ? row + q * kStep : col[0], c = RC ? col[i] : row + q * kStep;
+    const uint16_t* at = p + static_cast<uint64_t>(q) * kStep * pitch;
+    asm volatile("" : "+s"(at));  // a scalar: not one sum of it and the lane's offset kept for every q
+    const uint16_t* g = at + off[i];
+    if constexpr (FAST) g = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(at) + 2u * off[i]);
+    else g = (k0 + k < K) & (c0 + c < C) ? g : zero;  // (no branch)
+    __builtin_amdgcn_global_load_lds(g, (lds_void*)(lds + (q * WAVES + wave) * 512u), 16, 0, 0);
+  }
+};
+
+// Loads of the steps after step `at` up to step 0: qa in an even one, qb in an odd one.
+constexpr int loads_after(int at, int qa, int qb) {
+  int n = 0;
+  for (int s = at + 1; s <= 0; ++s) n += s % 2 == 0 ? qa : qb;
+  return n;
+}
 
 // A tile of BM x 2 HB (a pair: BM x HB of each product), WGM x WGN waves, each
 // (BM / WGM) rows by HB / WGN columns of either half, for operands whose rows
 // are whole chunks of 8 (K % 8 == 0 where K-contiguous, M or N % 8 == 0 where
 // row-contiguous).
 //
-// K advances in 32-deep slices through a ring of 4 slots of LDS, filled by
-// global_load_lds (lane i of a load writes 16 bytes at 16 i of a 1 KiB chunk,
-// from any global address: each lane's address is the inverse of the LDS
-// swizzle). Step t waits until slice t + 1 has landed and every read of slice
-// t has completed, one barrier, then runs the MFMAs of slice t on registers
-// while it reads the fragments of slice t + 1 into the other register set and
-// loads slice t + 4 into slice t's slot. Every step issues the same loads: a
-// chunk outside its operand, or past the last slice, is read from kZeroChunk,
-// so no tail of k, edge of the plane or border between segments needs code
-// of its own, and the count of loads in flight is static. (The operands are
-// __restrict__ parameters: without them the compiler takes a transposing read
-// of LDS to depend on every load into it and waits for all of them.)
-template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, uint32_t HB, uint32_t WGM, uint32_t WGN, typename Epi>
+// K advances in turns of 64 through rings of SA slots of A and SB of B, filled
+// by global_load_lds (lane i of a load writes 16 bytes at 16 i of a 1 KiB
+// chunk, from any global address: each lane's address is the inverse of the
+// LDS swizzle). 64 deep, a K-contiguous row is a whole 128-byte line of memory
+// (in slices of 32, loads of half lines cost 4096^3 of [M][K] by [N][K] a third of
+// its time), and one barrier serves two MFMA steps (a 128x128 tile needs 256
+// cycles for its MFMAs of 32 k and 450 for a barrier and the waits at it).
+// Turn t:
+//   step 0: MFMAs of k 0..31 on registers, while the fragments of k 32..63 are
+//           read into the other register set and A of turn t - 1 + SA is loaded
+//           into the slot of turn t - 1;
+//   wait until turn t + 1 has landed and every read of turn t has completed,
+//   barrier;
+//   step 1: MFMAs of k 32..63, reads of turn t + 1, k 0..31, and B of turn
+//           t + SB is loaded into the slot of turn t.
+// Every turn issues the same loads: a chunk outside its operand, or past the
+// last turn, is read from kZeroChunk, so no tail of k, edge of the plane or
+// border between segments needs code of its own, and the count of loads in
+// flight is static. (The operands are __restrict__ parameters: without them
+// the compiler takes a transposing read of LDS to depend on every load into it
+// and waits for all of them.)
+template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, uint32_t HB, uint32_t WGM, uint32_t WGN, int SA, int SB,
+          typename Epi>
 __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0, const uint16_t* __restrict__ pa1,
                                                 const uint16_t* __restrict__ pb00, const uint16_t* __restrict__ pb01,
                                                 const uint16_t* __restrict__ pb10, const uint16_t* __restrict__ pb11,
                                                 const uint16_t* __restrict__ zero, uint32_t M, uint32_t N, uint32_t K,
                                                 const Epi& epi, uint32_t tile) {
-  constexpr uint32_t WAVES = WGM * WGN, TM = BM / WGM, TH = HB / WGN, ASL = BM * 32u, BSL = HB * 32u, SLOT = ASL + 2u * BSL;
-  constexpr int IM = TM / 16, JH = TH / 16, JN = 2 * JH, QA = BM / 16 / WAVES, QB = 2 * HB / 16 / WAVES;
-  static_assert(BM / 16 % WAVES == 0 && 2 * HB / 16 % WAVES == 0 && HB / 16 % QB == 0, "whole chunks, of one half, per wave");
-  __shared__ __attribute__((aligned(16))) uint16_t lds[4 * SLOT];
+  constexpr uint32_t WAVES = WGM * WGN, TM = BM / WGM, TH = HB / WGN, ASL = BM * 64u, BSL = HB * 64u;
+  constexpr int IM = TM / 16, JH = TH / 16, JN = 2 * JH, QA = BM / 8 / WAVES, QB = 2 * HB / 8 / WAVES;
+  static_assert(BM / 8 % WAVES == 0 && HB / 8 % WAVES == 0, "whole chunks, of either half, per wave");
+  static_assert(SA >= 3 && SB >= 2, "A is loaded a turn later than B");
+  __shared__ __attribute__((aligned(16))) uint16_t lds[SA * ASL + SB * 2u * BSL];
   const uint32_t width = PAIR ? HB : 2u * HB;
   uint32_t tm, tn;
   gemm_tile_coords((M - 1u) / BM + 1u, (N - 1u) / width + 1u, &tm, &tn, tile);
   const uint32_t m0 = tm * BM, n0 = tn * width;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t wm = (wave / WGN) * TM, wn = (wave % WGN) * TH;
-  // This lane's place in each chunk that its wave fills: the offset from the
-  // panel's first element of a slice, its first k in the slice, and the end
-  // of k (0: the chunk lies outside the plane).
-  uint32_t offa[QA], ka[QA], enda[QA], offb[QB], kb[QB], endb[QB];
-#pragma unroll
-  for (int q = 0; q < QA; ++q) {
-    const uint32_t slot = (wave * QA + q) * 64u + lane;
-    if constexpr (A_RC) {
-      const uint32_t k = slot / (BM / 8u), m = ((slot % (BM / 8u)) ^ kn_slot_xor<BM>(k)) * 8u;
-      offa[q] = k * M + m;
-      ka[q] = k;
-      enda[q] = m0 + m < M ? K : 0u;
-    } else {
-      const uint32_t r = slot >> 2, c = (slot & 3u) ^ (((r >> 3) & 1u) << 1);
-      offa[q] = r * K + c * 8u;
-      ka[q] = c * 8u;
-      enda[q] = m0 + r < M ? K : 0u;
-    }
-  }
-  const uint32_t half = wave * QB * 16u / HB, nh = PAIR ? n0 : n0 + half * HB;  // the half that this wave fills
-#pragma unroll
-  for (int q = 0; q < QB; ++q) {
-    const uint32_t slot = (wave * QB + q) * 64u + lane - half * (BSL / 8u);
-    if constexpr (B_RC) {
-      const uint32_t k = slot / (HB / 8u), n = ((slot % (HB / 8u)) ^ kn_slot_xor<HB>(k)) * 8u;
-      offb[q] = k * N + n;
-      kb[q] = k;
-      endb[q] = nh + n < N ? K : 0u;
-    } else {
-      const uint32_t r = slot >> 2, c = (slot & 3u) ^ (((r >> 3) & 1u) << 1);
-      offb[q] = r * K + c * 8u;
-      kb[q] = c * 8u;
-      endb[q] = nh + r < N ? K : 0u;
-    }
-  }
-  const uint32_t ns = (K + 31u) / 32u, total = ns * SEGS;
+  const uint32_t pitch_a = A_RC ? M : K, pitch_b = B_RC ? N : K;
+  const Fill<A_RC, BM, WAVES> fill_a(wave, lane, pitch_a);
+  const Fill<B_RC, HB, WAVES> fill_b(wave, lane, pitch_b);
+  const uint32_t ns = (K + 63u) / 64u, total = ns * SEGS;
   uint16_t* ldsp = lds;
-  // Slices whose chunks all lie inside the operands, for a tile that does:
+  // Turns whose chunks all lie inside the operands, for a tile that does:
   // their loads take the panel's address from scalar registers and a 32-bit
   // offset a lane, with no test (which costs a tenth of the whole time).
   const bool inner = m0 + BM <= M && n0 + width <= N && M <= kInnerMost && N <= kInnerMost && K <= kInnerMost;
-  const uint32_t whole = !inner ? 0u : K % 32u == 0u ? total : SEGS == 1 ? K / 32u : 0u;
-  // Where slice t's panels start; past the last slice every chunk is zeros.
-  struct Slice {
-    const uint16_t *a, *b;
-    uint32_t k0, slot;
+  const uint32_t whole = !inner ? 0u : K % 64u == 0u ? total : SEGS == 1 ? K / 64u : 0u;
+  // The first k of turn t in its segment; past the last turn every chunk is zeros.
+  auto first_k = [&](uint32_t t) { return t < total ? (SEGS == 1 || t < ns ? t : t - ns) * 64u : K; };
+  auto load_a = [&](auto fast, uint32_t t, uint32_t slot, int q) {
+    const uint32_t k0 = first_k(t);
+    const uint16_t* p = (SEGS == 1 || t < ns ? pa0 : pa1) +
+                        (A_RC ? static_cast<uint64_t>(k0) * M + m0 : static_cast<uint64_t>(m0) * K + k0);
+    fill_a.template load<decltype(fast)::value>(p, zero, ldsp + slot / 2u, q, pitch_a, wave, k0, m0, K, M);
   };
-  auto slice = [&](uint32_t t) {
-    const uint32_t seg = SEGS == 1 || t < ns ? 0u : 1u;
-    Slice s;
-    s.k0 = t < total ? (t - seg * ns) * 32u : K;
-    s.slot = (t & 3u) * SLOT;
-    const uint64_t k = s.k0;
-    s.a = (seg == 0u ? pa0 : pa1) + (A_RC ? k * M + m0 : static_cast<uint64_t>(m0) * K + k);
-    const uint32_t h = PAIR ? half : 0u;
-    const uint16_t* b = h == 0u ? (seg == 0u ? pb00 : pb01) : (seg == 0u ? pb10 : pb11);
-    s.b = b + (B_RC ? k * N + nh : static_cast<uint64_t>(nh) * K + k);
-    return s;
+  auto load_b = [&](auto fast, uint32_t t, uint32_t slot, int q) {  // q < QB / 2: the first half
+    const uint32_t k0 = first_k(t), h = q / (QB / 2), nh = PAIR ? n0 : n0 + h * HB;
+    const uint16_t* b = (PAIR && h != 0u) ? (SEGS == 1 || t < ns ? pb10 : pb11) : (SEGS == 1 || t < ns ? pb00 : pb01);
+    const uint16_t* p = b + (B_RC ? static_cast<uint64_t>(k0) * N + nh : static_cast<uint64_t>(nh) * K + k0);
+    fill_b.template load<decltype(fast)::value>(p, zero, ldsp + slot / 2u + h * BSL, q % (QB / 2), pitch_b, wave, k0, nh, K, N);
   };
-  auto load_a = [&](auto fast, const Slice& s, int q) {
-    const uint16_t* g = s.a + offa[q];
-    if constexpr (decltype(fast)::value) g = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(s.a) + 2u * offa[q]);
-    else g = s.k0 + ka[q] < enda[q] ? g : zero;
-    __builtin_amdgcn_global_load_lds(g, (lds_void*)(ldsp + s.slot + (wave * QA + q) * 512u), 16, 0, 0);
-  };
-  auto load_b = [&](auto fast, const Slice& s, int q) {
-    const uint16_t* g = s.b + offb[q];
-    if constexpr (decltype(fast)::value) g = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(s.b) + 2u * offb[q]);
-    else g = s.k0 + kb[q] < endb[q] ? g : zero;
-    __builtin_amdgcn_global_load_lds(g, (lds_void*)(ldsp + s.slot + ASL + (wave * QB + q) * 512u), 16, 0, 0);
-  };
-  auto rd_a = [&](uint32_t t, uint32_t i) -> bf16x8 {
-    const uint16_t* As = ldsp + (t & 3u) * SLOT;
-    if constexpr (A_RC) return frag_b16_tr<BM>(As, wm + 16u * i, lane);
-    else return *reinterpret_cast<const bf16x8*>(&As[swz_rows32(wm + 16u * i + (lane & 15u), lane >> 4)]);
-  };
-  auto rd_b = [&](uint32_t t, uint32_t j) -> bf16x8 {  // j < JH: the first half
-    const uint16_t* Bs = ldsp + (t & 3u) * SLOT + ASL + (j / JH) * BSL;
-    const uint32_t n = wn + 16u * (j % JH);
-    if constexpr (B_RC) return frag_b16_tr<HB>(Bs, n, lane);
-    else return *reinterpret_cast<const bf16x8*>(&Bs[swz_rows32(n + (lane & 15u), lane >> 4)]);
+  const Frags<A_RC, BM, IM> frags_a(wm, lane);
+  const Frags<B_RC, HB, JH> frags_b(wn, lane);
+  auto rd_a = [&](uint32_t slot, int h, int i) { return frags_a.read(ldsp, slot, h, i); };
+  auto rd_b = [&](uint32_t slot, int h, int j) {  // j < JH: the first half
+    return frags_b.read(ldsp, slot + (j / JH) * 2u * BSL, h, j % JH);
   };
   f32x4_t acc[IM][JN];
 #pragma unroll
@@ -560,64 +595,76 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
   using Fast = std::true_type;
   using Checked = std::false_type;
   bf16x8 a0[IM], b0[JN], a1[IM], b1[JN];
-  constexpr int LOADS = QA + QB;
-  auto sync = [&]() {  // all but two slices have landed, this wave's LDS reads have completed
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(waitcnt_imm(2 * LOADS, 0));
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  };
-  auto step = [&](auto fast, uint32_t t, const bf16x8* ca, const bf16x8* cb, bf16x8* na, bf16x8* nb) {
-    sync();
-    const Slice s = slice(t + 4u);
+  // Loads that may be in flight at turn t's barrier: those issued after the
+  // later one of A and B of turn t + 1. With the steps numbered 2t and 2t + 1, A
+  // of turn j is issued in step 2 (j + 1 - SA), B in step 2 (j - SB) + 1.
+  constexpr int kAt = 4 - 2 * SA > 3 - 2 * SB ? 4 - 2 * SA : 3 - 2 * SB;
+  constexpr int kFlight = loads_after(kAt, QA, QB);
+  constexpr int kStart = (SA - 1) * QA + SB * QB;  // the first turns' loads
+  static_assert(kStart < 64, "vmcnt holds the loads in flight");
+  // One 32-deep step: the MFMAs of one register set, with the reads of the
+  // other and then `n` loads evenly over them but the last few: in a burst,
+  // four SIMDs ask for twice what LDS gives. MFMA c takes block (i, j), i
+  // snaking, so that consecutive ones share an operand; operands swapped, so
+  // that a lane ends with four columns of one row.
+  auto step = [&](const bf16x8* ca, const bf16x8* cb, auto&& rd, auto n, auto&& ld) {
+    constexpr int kOps = IM + JN + decltype(n)::value, kOver = IM * JN - 4;
     fence();
-    // MFMA c takes block (i, j), i snaking, so that consecutive ones share an
-    // operand. Operands swapped: a lane ends with four columns of one row.
 #pragma unroll
     for (int c = 0; c < IM * JN; ++c) {
       const int j = c / IM, i = (j & 1) ? IM - 1 - c % IM : c % IM;
       if constexpr (kAgpr) mfma16_bf16_acc<F16>(acc[i][j], cb[j], ca[i]);
       else acc[i][j] = mfma_16x16x32_16b<F16>(cb[j], ca[i], acc[i][j]);
       fence();
-      // The reads of the next fragments, then the loads, evenly over the MFMAs
-      // but the last few: in a burst, four SIMDs ask for twice what LDS gives.
-      constexpr int kOps = IM + JN + LOADS, kOver = IM * JN - 4;
       for (int o = c * kOps / kOver; o < (c + 1) * kOps / kOver && o < kOps; ++o) {
-        if (o < IM) na[o] = rd_a(t + 1u, o);
-        else if (o < IM + JN) nb[o - IM] = rd_b(t + 1u, o - IM);
-        else if (o < IM + JN + QA) load_a(fast, s, o - IM - JN);
-        else load_b(fast, s, o - IM - JN - QA);
+        if (o < IM + JN) rd(o);
+        else ld(o - IM - JN);
       }
       fence();
     }
   };
-  for (uint32_t t = 0; t < 4u; ++t) {
-    const Slice s = slice(t);
+  // The slots of turns t - 1, t and t + 1 (bytes of LDS), kept as scalars.
+  constexpr uint32_t kA = 2u * ASL, kB = 4u * BSL, kB0 = SA * kA;
+  uint32_t a_last = (SA - 1) * kA, a_this = 0u, a_next = kA, b_this = kB0, b_next = kB0 + kB;
+  auto turn = [&](auto fast, uint32_t t) {
+    step(a0, b0, [&](int o) { if (o < IM) a1[o] = rd_a(a_this, 1, o); else b1[o - IM] = rd_b(b_this, 1, o - IM); },
+         std::integral_constant<int, QA>{}, [&](int q) { load_a(fast, t + SA - 1, a_last, q); });
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(kFlight, 0));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    step(a1, b1, [&](int o) { if (o < IM) a0[o] = rd_a(a_next, 0, o); else b0[o - IM] = rd_b(b_next, 0, o - IM); },
+         std::integral_constant<int, QB>{}, [&](int q) { load_b(fast, t + SB, b_this, q); });
+    a_last = a_this;
+    a_this = a_next;
+    a_next = a_next == (SA - 1) * kA ? 0u : a_next + kA;
+    b_this = b_next;
+    b_next = b_next == kB0 + (SB - 1) * kB ? kB0 : b_next + kB;
+  };
 #pragma unroll
-    for (int q = 0; q < QA; ++q) load_a(Checked{}, s, q);
+  for (int t = 0; t < (SA - 1 > SB ? SA - 1 : SB); ++t) {
+    if (t < SA - 1)
 #pragma unroll
-    for (int q = 0; q < QB; ++q) load_b(Checked{}, s, q);
+      for (int q = 0; q < QA; ++q) load_a(Checked{}, t, t * kA, q);
+    if (t < SB)
+#pragma unroll
+      for (int q = 0; q < QB; ++q) load_b(Checked{}, t, kB0 + t * kB, q);
   }
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(waitcnt_imm(3 * LOADS, 0));
+  __builtin_amdgcn_s_waitcnt(waitcnt_imm(kStart - QA - QB, 0));
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < IM; ++i) a0[i] = rd_a(0u, i);
+  for (int i = 0; i < IM; ++i) a0[i] = rd_a(a_this, 0, i);
 #pragma unroll
-  for (int j = 0; j < JN; ++j) b0[j] = rd_b(0u, j);
-  // An odd count ends with a slice of zeros; K = 0 is two of them (a branch
-  // round the loop would hold the accumulators in two places, and spill).
+  for (int j = 0; j < JN; ++j) b0[j] = rd_b(b_this, 0, j);
+  // K = 0 is one turn of zeros (a branch round the loop would hold the
+  // accumulators in two places, and spill).
   uint32_t t = 0u;
-  for (; t + 5u < whole; t += 2u) {
-    step(Fast{}, t, a0, b0, a1, b1);
-    step(Fast{}, t + 1u, a1, b1, a0, b0);
-  }
-  do {
-    step(Checked{}, t, a0, b0, a1, b1);
-    step(Checked{}, t + 1u, a1, b1, a0, b0);
-    t += 2u;
-  } while (t < total);
+  constexpr uint32_t kAhead = SA - 1 > SB ? SA - 1 : SB;
+  for (; t + kAhead < whole; ++t) turn(Fast{}, t);
+  do turn(Checked{}, t++);
+  while (t < total);
   // No load into LDS is in flight past the loop, in any wave.
   __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
   __builtin_amdgcn_s_barrier();
@@ -633,9 +680,10 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
   else product_store<IM, JH, PAIR, false>(acc, own, m0 + wm, n0 + wn, HB, M, N, epi, lane);
 }
 
-template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, uint32_t HB, uint32_t WGM, uint32_t WGN, typename Epi>
+template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, uint32_t HB, uint32_t WGM, uint32_t WGN, int SA, int SB,
+          typename Epi>
 __device__ __forceinline__ void product_ring(const Operands<SEGS>& p, const Epi& epi, uint32_t tile) {
-  product_ring_of<F16, A_RC, B_RC, PAIR, SEGS, BM, HB, WGM, WGN>(
+  product_ring_of<F16, A_RC, B_RC, PAIR, SEGS, BM, HB, WGM, WGN, SA, SB>(
       p.a[0], p.a[SEGS - 1], p.b[0][0], p.b[0][SEGS - 1], p.b[1][0], p.b[1][SEGS - 1],
       reinterpret_cast<const uint16_t*>(kZeroChunk), p.M, p.N, p.K, epi, tile);
 }

@@ -343,7 +343,8 @@ def test_gated_backward_attributes(gpu, M, K, N, elem, attrs):
     check_gated_backward(elem, M, K, N, **attrs)
 
 
-@pytest.mark.parametrize("M,K,N", [(3592, 72, 3608), (3592, 264, 3600)])
+@pytest.mark.parametrize("M,K,N", [(3592, 72, 3608), (3592, 264, 3600), (2056, 72, 3080), (1032, 40, 3080), (1504, 72, 2904),
+                                   (1000, 40, 2304)])
 def test_large_planes(gpu, M, K, N):
     """Planes of many tiles, their last row and column of tiles partial, a
     reduction that ends inside a slice."""
