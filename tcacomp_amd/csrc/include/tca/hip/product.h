@@ -580,18 +580,17 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
 #pragma unroll
     for (int j = 0; j < JN; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   auto fence = []() { __builtin_amdgcn_sched_barrier(0); };
-  // 64 blocks a wave: the accumulators are tied to AGPRs by inline-asm MFMAs,
-  // with the hazards covered as at gemm_bf16_4w (the operands are results of
-  // LDS reads only; wait states before the first and after the last).
-  constexpr bool kAgpr = IM * JN >= 64;
-  if constexpr (kAgpr) {
+  // The accumulators are tied to AGPRs by inline-asm MFMAs (the compiler's own
+  // move them from one AGPR to another, 64 moves a turn of 128x128, and a third
+  // of the time at 256x128), with the hazards covered as at gemm_bf16_4w: the
+  // operands are results of LDS reads only; wait states before the first and
+  // after the last.
 #pragma unroll
-    for (int i = 0; i < IM; ++i)
+  for (int i = 0; i < IM; ++i)
 #pragma unroll
-      for (int j = 0; j < JN; ++j) asm volatile("" : "+a"(acc[i][j]));
-    asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
-    fence();
-  }
+    for (int j = 0; j < JN; ++j) asm volatile("" : "+a"(acc[i][j]));
+  asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
+  fence();
   using Fast = std::true_type;
   using Checked = std::false_type;
   bf16x8 a0[IM], b0[JN], a1[IM], b1[JN];
@@ -613,8 +612,7 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
 #pragma unroll
     for (int c = 0; c < IM * JN; ++c) {
       const int j = c / IM, i = (j & 1) ? IM - 1 - c % IM : c % IM;
-      if constexpr (kAgpr) mfma16_bf16_acc<F16>(acc[i][j], cb[j], ca[i]);
-      else acc[i][j] = mfma_16x16x32_16b<F16>(cb[j], ca[i], acc[i][j]);
+      mfma16_bf16_acc<F16>(acc[i][j], cb[j], ca[i]);
       fence();
       for (int o = c * kOps / kOver; o < (c + 1) * kOps / kOver && o < kOps; ++o) {
         if (o < IM + JN) rd(o);
@@ -669,11 +667,9 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
   __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  if constexpr (kAgpr) {
-    fence();
-    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
-    fence();
-  }
+  fence();
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+  fence();
   static_assert(WAVES * 64u * 2u * TH * 4u <= sizeof(lds), "64 rows of every wave");
   float* own = reinterpret_cast<float*>(lds) + wave * (64u * 2u * TH);
   if (m0 + BM <= M && n0 + width <= N) product_store<IM, JH, PAIR, true>(acc, own, m0 + wm, n0 + wn, HB, M, N, epi, lane);
