@@ -360,6 +360,11 @@ struct Product {
   std::string epi;                    // an expression of the epilogue's type
 };
 
+// Rows of a forward product that product_few takes, and its split of k: at
+// least kFewK of it for each workgroup that shares a strip, and no more
+// workgroups than kFewBlocks.
+constexpr uint32_t kFewRows = 64, kFewK = 256, kFewBlocks = 256;
+
 void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   std::ostringstream ops;
   ops << "  tca::hip::Operands<" << p.segs << "> p;\n";
@@ -375,12 +380,46 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   auto tiles = [&](uint32_t rows, uint32_t cols) {
     return p.M + "/" + std::to_string(rows) + " " + p.N + "/" + std::to_string(p.pair ? cols / 2u : cols);
   };
+  // A forward product of few rows, at any alignment.
+  const bool few = !p.a_rc && p.b_rc;
+  if (few) {
+    const std::string strips = "((N - 1u) / tca::hip::kFewColumns + 1u)";
+    const std::string P = "tca::hip::col_split(K, " + strips + ", " + std::to_string(kFewK) + "u, " + std::to_string(kFewBlocks) + "u)";
+    const std::string split = "split K " + std::to_string(kFewK) + " " + std::to_string(kFewBlocks) + " ";
+    w->Dim("few_parts", uint64_t{kFewBlocks} * 64u * kFewRows * (p.pair ? 2u : 1u));
+    w->Tensor("few_part", "f32", "local", "few_parts");
+    uint32_t from = 1;
+    for (uint32_t blocks : {1u, 2u, 4u}) {
+      Writer::Kernel k;
+      k.suffix = p.suffix + "_few" + std::to_string(16u * blocks);
+      k.params = p.params + " few_part";
+      k.block = 512;
+      k.body = ops.str() + "  tca::hip::product_few<" + f16 + ", " + Bool(p.pair) + ", " + std::to_string(blocks) + ">(p, epi, few_part, " +
+               strips + ", " + P + ");\n";
+      k.grid = "N/64";
+      k.records = {split + "0 1 N/64", When("M", from, 16u * blocks)};
+      k.detail = p.what + ", " + std::to_string(from) + " to " + std::to_string(16u * blocks) + " rows, strips of 64 columns, k over 8 waves and P workgroups";
+      w->Add(k);
+      from = 16u * blocks + 1u;
+    }
+    Writer::Kernel j;
+    j.suffix = p.suffix + "_fewjoin";
+    j.params = p.params + " few_part";
+    j.body = ops.str() + "  tca::hip::few_join<" + Bool(p.pair) + ">(few_part, epi, M, N, " + P + ");\n";
+    j.grid = "M/1 N/2048";
+    j.records = {split + "1 1 N/64", When("M", 1, kFewRows)};
+    j.detail = p.what + ", the partial sums of few rows (P > 1 only)";
+    w->Add(j);
+  }
+  const std::string many = When("M", kFewRows + 1u, kMost);
   // Rows of whole 16-byte chunks, of both operands, go straight into LDS.
   std::vector<std::string> aligned, odd;
   for (const std::string& d : std::set<std::string>{p.a_rc ? p.M : p.K, p.b_rc ? p.N : p.K}) {
     aligned.push_back(When(d, 0, kMost, 8));
     odd.push_back("unless " + d + " 0 " + std::to_string(kMost) + " 8 0");
   }
+  if (few) aligned.push_back(many);
+  if (few) odd.push_back(many);
   Writer::Kernel k;
   k.suffix = p.suffix + "_r";
   k.params = p.params;

@@ -684,6 +684,184 @@ __device__ __forceinline__ void product_ring(const Operands<SEGS>& p, const Epi&
       reinterpret_cast<const uint16_t*>(kZeroChunk), p.M, p.N, p.K, epi, tile);
 }
 
+// ----------------------------------------------- few rows: the weight is read
+// At most 64 rows of x [M][K] by a row-contiguous weight (of a pair: two): bound by
+// the weight's bytes. Nothing of it goes through LDS: a lane reads 4 columns
+// of the 8 rows of k that an MFMA operand holds, 16 lanes a whole 128-byte
+// line of a row, and transposes them in registers (one byte permute for two values);
+// column j of every lane makes one operand, so that operand's 16 columns are 4
+// apart, which the result only has to know. Eight waves of a workgroup take
+// every eighth 32-deep step of a strip of 64 columns and meet in LDS in wave
+// order; where strips are few, P workgroups share one, each a run of steps, and
+// few_join adds their partial sums in order (`part`, [P][1 or 2][M][N]).
+constexpr uint32_t kFewColumns = 64, kFewWaves = 8;
+
+typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+
+template <bool F16, bool PAIR, int MB, typename Epi>
+__device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi, float* __restrict__ part, uint32_t strips,
+                                            uint32_t P) {
+  constexpr int H = PAIR ? 2 : 1, D = MB == 4 ? 2 : 4;  // steps in registers
+  constexpr uint32_t PITCH = H * kFewColumns;
+  __shared__ __attribute__((aligned(16))) float lds[kFewWaves * 16u * PITCH];
+  const uint32_t M = p.M, N = p.N, K = p.K;
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t c = lane & 15u, g = lane >> 4, strip = blockIdx.x % strips, chunk = blockIdx.x / strips;
+  const uint32_t n0 = strip * kFewColumns, n = n0 + 4u * c;
+  // A lane's columns: past the end, the last four (stored where they are its own).
+  const uint32_t at = n + 4u <= N ? n : N >= 4u ? N - 4u : 0u;
+  const uint32_t ns = (K + 31u) / 32u, per = (ns + P - 1u) / P, first = chunk * per;
+  const uint32_t end = first + per < ns ? first + per : ns;
+  struct Step {
+    u32x2 w[H][8];
+    u32x4 x[MB];
+  };
+  Step st[D];
+  auto load = [&](Step& s, uint32_t t) {  // a step past the end re-reads the last rows; it is not used
+    const uint32_t k0 = t * 32u + 8u * g;
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (uint32_t e = 0; e < 8u; ++e) {
+        const uint32_t k = k0 + e < K ? k0 + e : K - 1u;
+        const uint16_t* row = p.b[h][0] + static_cast<uint64_t>(k) * N + at;
+        if (N >= 4u) {
+          s.w[h][e] = *reinterpret_cast<const u32x2_a2*>(row);
+        } else {
+          const u32x4 v = gather16(row, N);
+          s.w[h][e] = u32x2{v[0], v[1]};
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      const uint32_t m = 16u * i + c;
+      const uint16_t* row = p.a[0] + static_cast<uint64_t>(m < M ? m : M - 1u) * K;
+      if (K >= 8u) s.x[i] = load16_any(row + (k0 < K - 8u ? k0 : K - 8u));
+      else s.x[i] = gather16(row + (k0 < K ? k0 : 0u), k0 < K ? K - k0 : 0u);
+    }
+  };
+  f32x4_t acc[H][MB][4];
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[h][i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  auto compute = [&](Step& s, uint32_t t) {
+    const uint32_t k0 = t * 32u + 8u * g;
+    if (t * 32u + 32u > K) {  // the last, short step: zeros past K in both operands
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e)
+          if (k0 + e >= K) s.w[h][e] = u32x2{0u, 0u};
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+        if (K >= 8u && k0 + 8u > K) s.x[i] = shift_down16(s.x[i], k0 - (K - 8u));
+    }
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u32x4 w;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)  // k 2d and 2d + 1 of column j
+          w[d] = __builtin_amdgcn_perm(s.w[h][2 * d + 1][j / 2], s.w[h][2 * d][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+          acc[h][i][j] = mfma_16x16x32_16b<F16>(__builtin_bit_cast(bf16x8, s.x[i]), __builtin_bit_cast(bf16x8, w), acc[h][i][j]);
+      }
+  };
+  const uint32_t t0 = first + wave;
+  if (t0 < end) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(st[d], t0 + d * kFewWaves);
+    for (uint32_t t = t0; t < end; t += D * kFewWaves) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const uint32_t s = t + d * kFewWaves;
+        if (s < end) compute(st[d], s);
+        if (s + D * kFewWaves < end) load(st[d], s + D * kFewWaves);
+      }
+    }
+  }
+  // acc[h][i][j][e] is the sum of row 16 i + 4 g + e, column at + j.
+  const bool direct = P == 1u;
+#pragma unroll
+  for (int i = 0; i < MB; ++i) {
+    if (16u * i >= M) break;
+    if (i > 0) __syncthreads();
+    float* own = lds + wave * (16u * PITCH);
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (uint32_t e = 0; e < 4u; ++e) {
+        float* row = own + (4u * g + e) * PITCH + h * kFewColumns;
+        if (at == n) {
+          *reinterpret_cast<f32x4_t*>(row + 4u * c) = f32x4_t{acc[h][i][0][e], acc[h][i][1][e], acc[h][i][2][e], acc[h][i][3][e]};
+        } else if (n < N) {
+#pragma unroll
+          for (uint32_t j = 0; j < 4u; ++j)
+            if (at + j >= n && at + j < N) row[at + j - n0] = acc[h][i][j][e];
+        }
+      }
+    __syncthreads();
+    const uint32_t r = threadIdx.x >> 3, k = threadIdx.x & 7u, m = 16u * i + r, nk = n0 + 8u * k;
+    if (r < 16u && m < M && nk < N) {
+      float v[H][8];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[h][e] = 0.0f;
+        const float* from = lds + r * PITCH + h * kFewColumns + 8u * k;
+#pragma unroll
+        for (uint32_t w = 0; w < kFewWaves; ++w) {
+          const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(from + w * (16u * PITCH));
+          const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(from + w * (16u * PITCH) + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[h][e] += lo[e];
+            v[h][4 + e] += hi[e];
+          }
+        }
+      }
+      if (direct) {
+        const auto f = epi.template fetch<false>(m, nk);
+        if constexpr (PAIR) epi.template store<false>(m, nk, f, v[0], v[1]);
+        else epi.template store<false>(m, nk, f, v[0]);
+      } else {
+#pragma unroll
+        for (int h = 0; h < H; ++h) row_store<8>(part + (static_cast<uint64_t>(chunk * H + h) * M + m) * N, nk, N, v[h]);
+      }
+    }
+  }
+}
+
+// The P partial sums of eight columns a lane, in order, to the epilogue: 256
+// lanes a workgroup, along row blockIdx.x % M.
+template <bool PAIR, typename Epi>
+__device__ __forceinline__ void few_join(const float* __restrict__ part, const Epi& epi, uint32_t M, uint32_t N, uint32_t P) {
+  constexpr int H = PAIR ? 2 : 1;
+  const uint32_t m = blockIdx.x % M, n = (blockIdx.x / M * 256u + threadIdx.x) * 8u;
+  if (n >= N) return;
+  const auto f = epi.template fetch<false>(m, n);
+  float v[H][8];
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[h][e] = 0.0f;
+#pragma unroll 4
+    for (uint32_t p = 0; p < P; ++p) {
+      float s[8];
+      row_load<8>(part + (static_cast<uint64_t>(p * H + h) * M + m) * N, n, N, s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[h][e] += s[e];
+    }
+  }
+  if constexpr (PAIR) epi.template store<false>(m, n, f, v[0], v[1]);
+  else epi.template store<false>(m, n, f, v[0]);
+}
+
 // ------------------------------------------ gradients of the pre-activations
 // One element each: dz = dy act'(z) of a projection, dg = dh u act'(g) and
 // du = dh act(g) of a gated pair. i(e) is (dy, z) or (dh, g, u).
