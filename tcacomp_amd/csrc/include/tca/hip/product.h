@@ -488,7 +488,7 @@ struct Fill {
     asm volatile("" : "+s"(at));  // a scalar: not one sum of it and the lane's offset kept for every q
     const uint16_t* g = at + off[i];
     if constexpr (FAST) g = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(at) + 2u * off[i]);
-    else g = (k0 + k < K) & (c0 + c < C) ? g : zero;  // (no branch)
+    else g = ((k0 + k < K) & (c0 + c < C)) ? g : zero;  // (no branch)
     __builtin_amdgcn_global_load_lds(g, (lds_void*)(lds + (q * WAVES + wave) * 512u), 16, 0, 0);
   }
 };
@@ -696,24 +696,25 @@ __device__ __forceinline__ void product_ring(const Operands<SEGS>& p, const Epi&
 // few_join adds their partial sums in order (`part`, [P][1 or 2][M][N]).
 constexpr uint32_t kFewColumns = 64, kFewWaves = 8;
 
-typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
-
 template <bool F16, bool PAIR, int MB, typename Epi>
 __device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi, float* __restrict__ part, uint32_t strips,
                                             uint32_t P) {
-  constexpr int H = PAIR ? 2 : 1, D = MB == 4 ? 2 : 4;  // steps in registers
-  constexpr uint32_t PITCH = H * kFewColumns;
+  constexpr int H = PAIR ? 2 : 1, D = H * MB > 4 ? 2 : 4;  // steps in registers
+  constexpr int VEC = 4;                                   // columns a lane
+  constexpr uint32_t COLS = kFewColumns, PITCH = H * COLS, CHUNKS = COLS / 8u;
+  typedef uint32_t Row __attribute__((ext_vector_type(VEC / 2)));
+  typedef uint32_t RowAny __attribute__((ext_vector_type(VEC / 2), aligned(2)));
   __shared__ __attribute__((aligned(16))) float lds[kFewWaves * 16u * PITCH];
   const uint32_t M = p.M, N = p.N, K = p.K;
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t c = lane & 15u, g = lane >> 4, strip = blockIdx.x % strips, chunk = blockIdx.x / strips;
-  const uint32_t n0 = strip * kFewColumns, n = n0 + 4u * c;
-  // A lane's columns: past the end, the last four (stored where they are its own).
-  const uint32_t at = n + 4u <= N ? n : N >= 4u ? N - 4u : 0u;
+  const uint32_t n0 = strip * COLS, n = n0 + VEC * c;
+  // A lane's columns: past the end, the last VEC (stored where they are its own).
+  const uint32_t at = n + VEC <= N ? n : N >= VEC ? N - VEC : 0u;
   const uint32_t ns = (K + 31u) / 32u, per = (ns + P - 1u) / P, first = chunk * per;
   const uint32_t end = first + per < ns ? first + per : ns;
   struct Step {
-    u32x2 w[H][8];
+    Row w[H][8];
     u32x4 x[MB];
   };
   Step st[D];
@@ -725,11 +726,13 @@ __device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi
       for (uint32_t e = 0; e < 8u; ++e) {
         const uint32_t k = k0 + e < K ? k0 + e : K - 1u;
         const uint16_t* row = p.b[h][0] + static_cast<uint64_t>(k) * N + at;
-        if (N >= 4u) {
-          s.w[h][e] = *reinterpret_cast<const u32x2_a2*>(row);
+        if (N >= VEC) {
+          // Read once by the whole grid: not kept in the caches (5% of the time).
+          s.w[h][e] = __builtin_nontemporal_load(reinterpret_cast<const RowAny*>(row));
         } else {
           const u32x4 v = gather16(row, N);
-          s.w[h][e] = u32x2{v[0], v[1]};
+#pragma unroll
+          for (int d = 0; d < VEC / 2; ++d) s.w[h][e][d] = v[d];
         }
       }
 #pragma unroll
@@ -740,13 +743,13 @@ __device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi
       else s.x[i] = gather16(row + (k0 < K ? k0 : 0u), k0 < K ? K - k0 : 0u);
     }
   };
-  f32x4_t acc[H][MB][4];
+  f32x4_t acc[H][MB][VEC];
 #pragma unroll
   for (int h = 0; h < H; ++h)
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[h][i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int j = 0; j < VEC; ++j) acc[h][i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   auto compute = [&](Step& s, uint32_t t) {
     const uint32_t k0 = t * 32u + 8u * g;
     if (t * 32u + 32u > K) {  // the last, short step: zeros past K in both operands
@@ -754,7 +757,9 @@ __device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi
       for (int h = 0; h < H; ++h)
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e)
-          if (k0 + e >= K) s.w[h][e] = u32x2{0u, 0u};
+#pragma unroll
+          for (int d = 0; d < VEC / 2; ++d)
+            if (k0 + e >= K) s.w[h][e][d] = 0u;
 #pragma unroll
       for (int i = 0; i < MB; ++i)
         if (K >= 8u && k0 + 8u > K) s.x[i] = shift_down16(s.x[i], k0 - (K - 8u));
@@ -762,7 +767,7 @@ __device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < VEC; ++j) {
         u32x4 w;
 #pragma unroll
         for (int d = 0; d < 4; ++d)  // k 2d and 2d + 1 of column j
@@ -796,24 +801,27 @@ __device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi
     for (int h = 0; h < H; ++h)
 #pragma unroll
       for (uint32_t e = 0; e < 4u; ++e) {
-        float* row = own + (4u * g + e) * PITCH + h * kFewColumns;
+        float* row = own + (4u * g + e) * PITCH + h * COLS;
         if (at == n) {
-          *reinterpret_cast<f32x4_t*>(row + 4u * c) = f32x4_t{acc[h][i][0][e], acc[h][i][1][e], acc[h][i][2][e], acc[h][i][3][e]};
+#pragma unroll
+          for (int j = 0; j < VEC; j += 4)
+            *reinterpret_cast<f32x4_t*>(row + VEC * c + j) =
+                f32x4_t{acc[h][i][j][e], acc[h][i][j + 1][e], acc[h][i][j + 2][e], acc[h][i][j + 3][e]};
         } else if (n < N) {
 #pragma unroll
-          for (uint32_t j = 0; j < 4u; ++j)
+          for (uint32_t j = 0; j < VEC; ++j)
             if (at + j >= n && at + j < N) row[at + j - n0] = acc[h][i][j][e];
         }
       }
     __syncthreads();
-    const uint32_t r = threadIdx.x >> 3, k = threadIdx.x & 7u, m = 16u * i + r, nk = n0 + 8u * k;
+    const uint32_t r = threadIdx.x / CHUNKS, k = threadIdx.x % CHUNKS, m = 16u * i + r, nk = n0 + 8u * k;
     if (r < 16u && m < M && nk < N) {
       float v[H][8];
 #pragma unroll
       for (int h = 0; h < H; ++h) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[h][e] = 0.0f;
-        const float* from = lds + r * PITCH + h * kFewColumns + 8u * k;
+        const float* from = lds + r * PITCH + h * COLS + 8u * k;
 #pragma unroll
         for (uint32_t w = 0; w < kFewWaves; ++w) {
           const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(from + w * (16u * PITCH));
@@ -847,16 +855,22 @@ __device__ __forceinline__ void few_join(const float* __restrict__ part, const E
   const auto f = epi.template fetch<false>(m, n);
   float v[H][8];
 #pragma unroll
-  for (int h = 0; h < H; ++h) {
+  for (int h = 0; h < H; ++h)
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[h][e] = 0.0f;
-#pragma unroll 4
-    for (uint32_t p = 0; p < P; ++p) {
-      float s[8];
-      row_load<8>(part + (static_cast<uint64_t>(p * H + h) * M + m) * N, n, N, s);
+  for (uint32_t p = 0; p < P; p += 4u) {  // four at a time in flight; past the end, the last one again
+    float s[4][H][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[h][e] += s[e];
-    }
+    for (uint32_t i = 0; i < 4u; ++i)
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+        row_load<8>(part + (static_cast<uint64_t>((p + i < P ? p + i : P - 1u) * H + h) * M + m) * N, n, N, s[i][h]);
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i)
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[h][e] = p + i < P ? v[h][e] + s[i][h][e] : v[h][e];
   }
   if constexpr (PAIR) epi.template store<false>(m, n, f, v[0], v[1]);
   else epi.template store<false>(m, n, f, v[0]);
