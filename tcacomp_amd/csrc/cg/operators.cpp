@@ -210,6 +210,7 @@ constexpr uint64_t kMost = 4294967295ull;
 // ------------------------------------------------------------- layer norm
 
 // The lanes and vectors that hold a row, by its length in 16-byte vectors.
+constexpr uint32_t kLanes = 256 * 2048;  // of the card
 struct RowForm {
   uint32_t lanes, vectors;
   uint32_t Span() const { return lanes * vectors; }
@@ -238,6 +239,8 @@ void EmitLayerNorm(const Attrs& a, Writer* w) {
   uint64_t from = 0;
   for (const RowForm& f : {RowForm{16, 1}, RowForm{64, 1}, RowForm{64, 2}, RowForm{64, 4}, RowForm{256, 2},
                            RowForm{256, 4}, RowForm{1024, 2}, RowForm{1024, 4}}) {
+    // 16 waves have 128 registers each: 16-bit rows with f32 weights would spill.
+    if (f.Span() == 4096u && a.elem != a.weight) continue;
     const uint64_t to = static_cast<uint64_t>(f.Span()) * E;
     const uint32_t block = f.lanes < 256u ? 256u : f.lanes;
     const std::string g = std::to_string(f.lanes), v = std::to_string(f.vectors);
@@ -246,7 +249,8 @@ void EmitLayerNorm(const Attrs& a, Writer* w) {
     k.params = params;
     k.block = block;
     k.body = "  tca::hip::norm_rows<" + T + ", " + W + ", " + g + ", " + v + tail;
-    k.grid = "R/" + std::to_string(block / f.lanes);
+    // as many workgroups as the card holds at once, at most
+    k.grid = "R/" + std::to_string(block / f.lanes) + ":" + std::to_string(kLanes / block);
     k.records = {When("C", from, to)};
     k.detail = "rows of " + std::to_string(from) + " to " + std::to_string(to) + " in registers, " + g + " lanes of " + v + " vectors";
     w->Add(k);
@@ -296,20 +300,22 @@ void EmitLayerNormBackward(const Attrs& a, Writer* w) {
     j.params = part + " dgamma " + (bias ? "dbeta " : "") + "R C";
     j.body = "  tca::hip::join_partials<" + W + ">(" + part + ", dgamma, " + (bias ? "dbeta" : "(" + W + "*)nullptr") + ", " +
              (bias ? "2u" : "1u") + ", C, tca::hip::partial_rows(R, " + std::to_string(groups) + "u, " + std::to_string(most) + "u));\n";
+    j.block = 1024;
     j.grid = std::string("C/32") + (bias ? " 2/1" : "");
     j.records = {When("C", lo, hi)};
     j.detail = "the weights' gradients from the partial rows of " + std::to_string(groups) + " at a time";
     w->Add(j);
   };
   for (const RowForm& f : {RowForm{16, 1}, RowForm{64, 1}, RowForm{64, 2}, RowForm{256, 1}, RowForm{256, 2},
-                           RowForm{1024, 1}, RowForm{1024, 2}}) {
+                           RowForm{512, 2}, RowForm{512, 4}}) {
+    if (f.vectors == 4u && E == 8u) continue;  // two rows, their sums and the gradients' do not fit 256 registers
     const uint64_t to = static_cast<uint64_t>(f.Span()) * E;
-    const uint32_t groups = 1024u / f.lanes;
+    const uint32_t groups = 512u / f.lanes;
     const std::string g = std::to_string(f.lanes), v = std::to_string(f.vectors);
     Writer::Kernel k;
     k.suffix = "_" + g + "x" + v;
     k.params = ins + "part R C";
-    k.block = 1024;
+    k.block = 512;
     k.body = "  tca::hip::norm_backward_rows<" + T + ", " + W + ", " + g + ", " + v + ", " + Bool(bias) + ", " + Bool(res) +
              ">" + args + "part, R, C);\n";
     k.grid = "R/" + std::to_string(groups) + ":" + std::to_string(kParts);
@@ -543,6 +549,7 @@ void EmitBackward(const Attrs& a, bool gated, Writer* w) {
     j.suffix = "_bias";
     j.params = std::string("bias_part ") + (gated ? "dbg dbu " : "db ") + "M N";
     j.body = "  tca::hip::join_partials<" + T + ">(bias_part, " + (gated ? "dbg, dbu, 2u" : "db, " + none + ", 1u") + ", N, " + parts + ");\n";
+    j.block = 1024;
     j.grid = std::string("N/32") + (gated ? " 2/1" : "");
     j.detail = "the bias' gradient from its partial sums";
     w->Add(j);

@@ -26,70 +26,96 @@
 namespace tca {
 namespace hip {
 
-// The sum of v over the G lanes of a group; G > 64: over the G / 64 waves of
-// it too, through `lds` (one slot per wave of the workgroup). `lds` must not
-// be written again before a barrier: callers alternate between two.
-template <int G>
-__device__ __forceinline__ float norm_group_sum(float v, float* lds) {
-  v = seg_allreduce<(G < 64 ? G : 64)>(v, [](float a, float b) { return a + b; });
+// The sums of v[0] .. v[S - 1] over the G lanes of a group; G > 64: over the G /
+// 64 waves of it too, through `lds` (S floats for each wave of the workgroup).
+// `lds` must not be written again before a barrier: callers alternate
+// between two.
+template <int G, int S>
+__device__ __forceinline__ void norm_group_sums(float (&v)[S], float* lds) {
+#pragma unroll
+  for (int i = 0; i < S; ++i) v[i] = seg_allreduce<(G < 64 ? G : 64)>(v[i], [](float a, float b) { return a + b; });
   if constexpr (G > 64) {
     constexpr uint32_t kWaves = G / 64;
-    if (lane_id() == 0u) lds[wave_id()] = v;
-    __syncthreads();
-    const float* g = lds + wave_id() / kWaves * kWaves;
-    v = g[0];
 #pragma unroll
-    for (uint32_t i = 1; i < kWaves; ++i) v += g[i];
+    for (int i = 0; i < S; ++i)
+      if (lane_id() == 0u) lds[wave_id() * S + i] = v[i];
+    __syncthreads();
+    const float* g = lds + wave_id() / kWaves * kWaves * S;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      v[i] = g[i];
+#pragma unroll
+      for (uint32_t k = 1; k < kWaves; ++k) v[i] += g[k * S + i];
+    }
   }
-  return v;
 }
 
-// One row per group of G lanes, at most NV vectors per lane (C <= G NV E).
+// Rows by groups of G lanes, at most NV vectors per lane (C <= G NV E), the
+// workgroups walking them with the grid as their stride: a row's loads are
+// issued a row ahead, and gamma and beta are read once.
 template <typename T, typename W, int G, int NV, bool BIAS, bool STATS>
 __device__ __forceinline__ void norm_rows(const T* x, const W* __restrict__ gamma, const W* __restrict__ beta, T* y,
                                           float* __restrict__ mean, float* __restrict__ rstd, uint32_t R, uint32_t C,
                                           float eps) {
-  constexpr int E = kRowE<T>, BLOCK = G < 256 ? 256 : G;
-  __shared__ float lds[2][BLOCK / 64];
-  const uint32_t lane = threadIdx.x % G, row = blockIdx.x * (BLOCK / G) + threadIdx.x / G;
-  const bool live = row < R;
-  const uint64_t at = static_cast<uint64_t>(live ? row : 0u) * C;
-  float v[NV][E];
-  float s = 0.0f;
+  constexpr int E = kRowE<T>, BLOCK = G < 256 ? 256 : G, GROUPS = BLOCK / G;
+  __shared__ float lds[2][2][BLOCK / 64];
+  const uint32_t lane = threadIdx.x % G;
+  uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * GROUPS;  // the workgroup's first row
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * GROUPS, grp = threadIdx.x / G;
+  vec<T, E> next[NV];
+  vec<W, E> g[NV], b[NV];
+  auto load = [&](uint64_t row) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) next[i] = row_raw<E>(x + row * C, (i * G + lane) * E, C);
+  };
+  if (r0 + grp < R) load(r0 + grp);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    row_load<E>(x + at, (i * G + lane) * E, C, v[i]);
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += v[i][e];
+    g[i] = row_vec<E>(gamma, (i * G + lane) * E, C);
+    if constexpr (BIAS) b[i] = row_vec<E>(beta, (i * G + lane) * E, C);
   }
-  const float m = norm_group_sum<G>(s, lds[0]) / static_cast<float>(C);
-  float q = 0.0f;
+  // r0 is the same for every group: all of them reach the barriers.
+  for (uint32_t turn = 0u; r0 < R; r0 += step, ++turn) {
+    const uint64_t row = r0 + grp;
+    float v[NV][E];
+    float s[1] = {0.0f}, q[1] = {0.0f};
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      row_fix<E>(next[i], (i * G + lane) * E, C);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      v[i][e] -= m;
-      if ((i * G + lane) * E + e < C) q = __builtin_fmaf(v[i][e], v[i][e], q);
+      for (int e = 0; e < E; ++e) v[i][e] = static_cast<float>(next[i][e]);
     }
-  const float r = 1.0f / __builtin_sqrtf(norm_group_sum<G>(q, lds[1]) / static_cast<float>(C) + eps);
-  if (!live) return;
+    if (row + step < R) load(row + step);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t c = (i * G + lane) * E;
-    float g[E], b[E];
-    row_load<E>(gamma, c, C, g);
-    if constexpr (BIAS) row_load<E>(beta, c, C, b);
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      v[i][e] = v[i][e] * r * g[e];
-      if constexpr (BIAS) v[i][e] += b[e];
+      for (int e = 0; e < E; ++e) s[0] += v[i][e];
+    norm_group_sums<G>(s, lds[turn & 1u][0]);
+    const float m = s[0] / static_cast<float>(C);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        v[i][e] -= m;
+        if ((i * G + lane) * E + e < C) q[0] = __builtin_fmaf(v[i][e], v[i][e], q[0]);
+      }
+    norm_group_sums<G>(q, lds[turn & 1u][1]);
+    const float r = 1.0f / __builtin_sqrtf(q[0] / static_cast<float>(C) + eps);
+    if (row >= R) continue;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        v[i][e] = v[i][e] * r * static_cast<float>(g[i][e]);
+        if constexpr (BIAS) v[i][e] += static_cast<float>(b[i][e]);
+      }
+      row_store<E>(y + row * C, (i * G + lane) * E, C, v[i]);
     }
-    row_store<E>(y + at, c, C, v[i]);
-  }
-  if constexpr (STATS) {
-    if (lane == 0u) {
-      mean[row] = m;
-      rstd[row] = r;
+    if constexpr (STATS) {
+      if (lane == 0u) {
+        mean[row] = m;
+        rstd[row] = r;
+      }
     }
   }
 }
@@ -156,66 +182,87 @@ __device__ __forceinline__ void norm_long(const T* x, const W* __restrict__ gamm
 
 // ------------------------------------------------------------- backward pass
 
-// Workgroups of 1024 lanes, 1024 / G groups; `part` is [workgroups][1 + BIAS][C].
+// Workgroups of 512 lanes, 512 / G groups, walking the rows with the grid as
+// their stride, a row's loads issued a row ahead; `part` is [workgroups][1 + BIAS][C].
 template <typename T, typename W, int G, int NV, bool BIAS, bool RES>
 __device__ __forceinline__ void norm_backward_rows(const T* __restrict__ dy, const T* __restrict__ x,
                                                    const W* __restrict__ gamma, const float* __restrict__ mean,
                                                    const float* __restrict__ rstd, const T* dres, T* dx,
                                                    float* __restrict__ part, uint32_t R, uint32_t C) {
-  constexpr int E = kRowE<T>, BLOCK = 1024, GROUPS = BLOCK / G;
+  constexpr int E = kRowE<T>, BLOCK = 512, GROUPS = BLOCK / G;
   constexpr uint32_t SPAN = G * NV * E;
-  __shared__ float sums[2][2][BLOCK / 64];
+  __shared__ float sums[2][2 * BLOCK / 64];
   __shared__ __attribute__((aligned(16))) float join[GROUPS * SPAN];
   const uint32_t lane = threadIdx.x % G, grp = threadIdx.x / G;
   const float inv = 1.0f / static_cast<float>(C);
+  struct Row {
+    vec<T, E> x[NV], dy[NV], res[RES ? NV : 1];
+    float m, rs;
+  };
+  uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * GROUPS;
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * GROUPS;
+  auto load = [&](Row& w, uint64_t row) {
+    w.m = mean[row];
+    w.rs = rstd[row];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (i * G + lane) * E;
+      w.x[i] = row_raw<E>(x + row * C, c, C);
+      w.dy[i] = row_raw<E>(dy + row * C, c, C);
+      // dres may be dx: this row's elements are written by the lanes that read them.
+      if constexpr (RES) w.res[i] = row_raw<E>(dres + row * C, c, C);
+    }
+  };
+  Row next;
+  if (r0 + grp < R) load(next, r0 + grp);
+  vec<W, E> g[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) g[i] = row_vec<E>(gamma, (i * G + lane) * E, C);
   float dg[NV][E], db[NV][E];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < E; ++e) dg[i][e] = db[i][e] = 0.0f;
-  uint32_t turn = 0u;
-  // r0 < R is the same for every group: all of them reach the barriers.
-  for (uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * GROUPS; r0 < R; r0 += static_cast<uint64_t>(gridDim.x) * GROUPS) {
+  // r0 is the same for every group: all of them reach the barriers.
+  for (uint32_t turn = 0u; r0 < R; r0 += step, ++turn) {
     const uint64_t row = r0 + grp;
     const bool live = row < R;
-    const uint64_t at = live ? row * C : 0u;
-    const float m = live ? mean[row] : 0.0f, rs = live ? rstd[row] : 0.0f;
-    float h[NV][E], t[NV][E];
-    float s1 = 0.0f, s2 = 0.0f;
+    Row now = next;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (i * G + lane) * E;
-      float g[E];
-      row_load<E>(x + at, c, C, h[i]);
-      row_load<E>(dy + at, c, C, t[i]);
-      row_load<E>(gamma, c, C, g);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        h[i][e] = (h[i][e] - m) * rs;
-        if (live) {  // a group past the last row adds nothing, whatever row 0 holds
-          dg[i][e] = __builtin_fmaf(t[i][e], h[i][e], dg[i][e]);
-          db[i][e] += t[i][e];
-        }
-        t[i][e] *= g[e];
-        s1 += t[i][e];
-        if (c + e < C) s2 = __builtin_fmaf(t[i][e], h[i][e], s2);
-      }
+      row_fix<E>(now.x[i], c, C);
+      row_fix<E>(now.dy[i], c, C);
+      if constexpr (RES) row_fix<E>(now.res[i], c, C);
     }
-    s1 = norm_group_sum<G>(s1, sums[turn & 1u][0]);
-    s2 = norm_group_sum<G>(s2, sums[turn & 1u][1]);
-    ++turn;
+    if (row + step < R) load(next, row + step);
+    float s[2] = {0.0f, 0.0f};
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float h = (static_cast<float>(now.x[i][e]) - now.m) * now.rs, d = static_cast<float>(now.dy[i][e]);
+          dg[i][e] = __builtin_fmaf(d, h, dg[i][e]);
+          db[i][e] += d;
+          const float t = d * static_cast<float>(g[i][e]);
+          s[0] += t;
+          if ((i * G + lane) * E + e < C) s[1] = __builtin_fmaf(t, h, s[1]);
+        }
+    }
+    norm_group_sums<G>(s, sums[turn & 1u]);
     if (!live) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t c = (i * G + lane) * E;
       float o[E];
-      if constexpr (RES) row_load<E>(dres + at, c, C, o);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float d = (t[i][e] - (s1 + h[i][e] * s2) * inv) * rs;
-        o[e] = RES ? d + o[e] : d;
+        const float h = (static_cast<float>(now.x[i][e]) - now.m) * now.rs;
+        const float t = static_cast<float>(now.dy[i][e]) * static_cast<float>(g[i][e]);
+        o[e] = (t - (s[0] + h * s[1]) * inv) * now.rs;
+        if constexpr (RES) o[e] += static_cast<float>(now.res[i][e]);
       }
-      row_store<E>(dx + at, c, C, o);
+      row_store<E>(dx + row * C, (i * G + lane) * E, C, o);
     }
   }
   // The groups' sums, in group order.
@@ -245,7 +292,7 @@ __device__ __forceinline__ void norm_backward_long(const T* __restrict__ dy, con
                                                    const float* __restrict__ rstd, const T* dres, T* dx, uint32_t R,
                                                    uint32_t C) {
   constexpr int E = kRowE<T>;
-  __shared__ float sums[2][16];
+  __shared__ float sums[2 * 16];
   const uint32_t row = blockIdx.x;
   if (row >= R) return;
   const uint64_t at = static_cast<uint64_t>(row) * C;
@@ -262,8 +309,10 @@ __device__ __forceinline__ void norm_backward_long(const T* __restrict__ dy, con
       if (c + e < C) s2 = __builtin_fmaf(t[e] * g[e], (h[e] - m) * rs, s2);
     }
   }
-  s1 = norm_group_sum<1024>(s1, sums[0]);
-  s2 = norm_group_sum<1024>(s2, sums[1]);
+  float both[2] = {s1, s2};
+  norm_group_sums<1024>(both, sums);
+  s1 = both[0];
+  s2 = both[1];
   for (uint32_t c = threadIdx.x * E; c < C; c += 1024u * E) {
     float h[E], t[E], g[E], o[E];
     row_load<E>(x + at, c, C, h);

@@ -102,8 +102,8 @@ struct LinearStore {
   template <bool WHOLE>
   __device__ __forceinline__ Fetch fetch(uint32_t m, uint32_t n) const {
     Fetch f;
-    if constexpr (RES) f.res = row_raw<8, WHOLE>(res + static_cast<uint64_t>(m) * N, n, N);
-    if constexpr (BIAS) f.b = row_raw<8, WHOLE>(b, n, N);
+    if constexpr (RES) f.res = row_vec<8, WHOLE>(res + static_cast<uint64_t>(m) * N, n, N);
+    if constexpr (BIAS) f.b = row_vec<8, WHOLE>(b, n, N);
     return f;
   }
   template <bool WHOLE>
@@ -137,8 +137,8 @@ struct GatedStore {
   __device__ __forceinline__ Fetch fetch(uint32_t, uint32_t n) const {
     Fetch f;
     if constexpr (BIAS) {
-      f.bg = row_raw<8, WHOLE>(bg, n, N);
-      f.bu = row_raw<8, WHOLE>(bu, n, N);
+      f.bg = row_vec<8, WHOLE>(bg, n, N);
+      f.bu = row_vec<8, WHOLE>(bu, n, N);
     }
     return f;
   }
@@ -878,7 +878,7 @@ __device__ __forceinline__ void few_join(const float* __restrict__ part, const E
 
 // ------------------------------------------ gradients of the pre-activations
 // One element each: dz = dy act'(z) of a projection, dg = dh u act'(g) and
-// du = dh act(g) of a gated pair. i(e) is (dy, z) or (dh, g, u).
+// du = dh act(g) of a gated pair.
 template <typename T, int ACT, bool GATED>
 struct Slope {
   const T* dy;
@@ -886,26 +886,38 @@ struct Slope {
   const T* u;
   T* dz;  // dg of a pair; no store where ACT is none
   T* du;
-  // The vector at `at` (its E values before `end`): f0 = dz or dg, f1 = du.
-  template <int E>
-  __device__ __forceinline__ void operator()(uint64_t at, uint32_t c, uint32_t C, float (&f0)[E], float (&f1)[E]) const {
-    float a[E], b[E], d[E];
-    row_load<E>(dy + at, c, C, d);
-    if constexpr (ACT != kActNone || GATED) row_load<E>(z + at, c, C, a);
-    if constexpr (GATED) row_load<E>(u + at, c, C, b);
+  static constexpr bool kZ = ACT != kActNone || GATED;
+  struct Raw {
+    vec<T, 8> dy, z, u;
+  };
+  // The vector from element c of the row at `at`, of C.
+  __device__ __forceinline__ Raw load(uint64_t at, uint32_t c, uint32_t C) const {
+    Raw r;
+    r.dy = row_raw<8>(dy + at, c, C);
+    if constexpr (kZ) r.z = row_raw<8>(z + at, c, C);
+    if constexpr (GATED) r.u = row_raw<8>(u + at, c, C);
+    return r;
+  }
+  // f0 = dz or dg, f1 = du, stored.
+  __device__ __forceinline__ void store(Raw r, uint64_t at, uint32_t c, uint32_t C, float (&f0)[8], float (&f1)[8]) const {
+    row_fix<8>(r.dy, c, C);
+    if constexpr (kZ) row_fix<8>(r.z, c, C);
+    if constexpr (GATED) row_fix<8>(r.u, c, C);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
+    for (int e = 0; e < 8; ++e) {
+      const float d = static_cast<float>(r.dy[e]);
       if constexpr (GATED) {
-        f0[e] = d[e] * b[e] * act_slope<ACT>(a[e]);
-        f1[e] = d[e] * act<ACT>(a[e]);
+        const float a = static_cast<float>(r.z[e]);
+        f0[e] = d * static_cast<float>(r.u[e]) * act_slope<ACT>(a);
+        f1[e] = d * act<ACT>(a);
       } else if constexpr (ACT != kActNone) {
-        f0[e] = d[e] * act_slope<ACT>(a[e]);
+        f0[e] = d * act_slope<ACT>(static_cast<float>(r.z[e]));
       } else {
-        f0[e] = d[e];
+        f0[e] = d;
       }
     }
-    if constexpr (GATED || ACT != kActNone) row_store<E>(dz + at, c, C, f0);
-    if constexpr (GATED) row_store<E>(du + at, c, C, f1);
+    if constexpr (kZ) row_store<8>(dz + at, c, C, f0);
+    if constexpr (GATED) row_store<8>(du + at, c, C, f1);
   }
 };
 
@@ -915,15 +927,16 @@ __device__ __forceinline__ void slope_flat(const Slope<T, ACT, GATED>& f, uint32
   const uint32_t c = (blockIdx.x * 256u + threadIdx.x) * 8u;
   if (c >= n) return;
   float f0[8], f1[8];
-  f(0u, c, n, f0, f1);
+  f.store(f.load(0u, c, n), 0u, c, n, f0, f1);
 }
 
 // ... with the column sums of a bias' gradient, of the values before they are
-// rounded: 512 columns by 4 rows a workgroup, over row chunk p of P; `part`
-// is [P][1 + GATED][N].
+// rounded: 512 columns by 4 rows a workgroup, over row chunk p of P, four rows
+// of a lane in flight; `part` is [P][1 + GATED][N].
 template <typename T, int ACT, bool GATED>
 __device__ __forceinline__ void slope_columns(const Slope<T, ACT, GATED>& f, float* __restrict__ part, uint32_t M,
                                               uint32_t N, uint32_t P) {
+  constexpr uint32_t AHEAD = 4;
   __shared__ float join[4][512];
   const uint32_t p = blockIdx.x % P, c0 = blockIdx.x / P * 512u, c = c0 + lane_id() * 8u, slot = wave_id();
   const uint64_t rows = (M - 1u) / P + 1u, first = p * rows, last = first + rows < M ? first + rows : M;
@@ -931,13 +944,21 @@ __device__ __forceinline__ void slope_columns(const Slope<T, ACT, GATED>& f, flo
 #pragma unroll
   for (int e = 0; e < 8; ++e) s0[e] = s1[e] = 0.0f;
   if (c < N)
-    for (uint64_t r = first + slot; r < last; r += 4u) {
-      float f0[8], f1[8];
-      f(r * N, c, N, f0, f1);
+    for (uint64_t r = first + slot; r < last; r += 4u * AHEAD) {
+      typename Slope<T, ACT, GATED>::Raw raw[AHEAD];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        s0[e] += f0[e];
-        if constexpr (GATED) s1[e] += f1[e];
+      for (uint32_t k = 0; k < AHEAD; ++k)
+        if (r + 4u * k < last) raw[k] = f.load((r + 4u * k) * N, c, N);
+#pragma unroll
+      for (uint32_t k = 0; k < AHEAD; ++k) {
+        if (r + 4u * k >= last) break;
+        float f0[8], f1[8];
+        f.store(raw[k], (r + 4u * k) * N, c, N, f0, f1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          s0[e] += f0[e];
+          if constexpr (GATED) s1[e] += f1[e];
+        }
       }
     }
   constexpr uint32_t Q = GATED ? 2u : 1u;

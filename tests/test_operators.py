@@ -146,12 +146,12 @@ def test_partial_rows_are_as_many_as_the_join_adds():
         t = [desc("bf16", R, C), desc("bf16", R, C), desc("bf16", C), desc("f32", R), desc("f32", R), desc("bf16", R, C),
              desc("bf16", C), desc("bf16", C)]
         grids = selected(p, t)
-        if C > 16384:
+        if C > 8192:
             parts = min(-(-R // 64), 32)
             assert grids["tca_" + p.name + "_columns"] == -(-C // 512) * parts
         else:
             (lanes, grid), = [(int(s.rsplit("_", 1)[1].split("x")[0]), g) for s, g in grids.items() if not s.endswith("join")]
-            assert grid == min(-(-R // (1024 // lanes)), 256)
+            assert grid == min(-(-R // (512 // lanes)), 256)
 
 
 def test_shape_contract():
