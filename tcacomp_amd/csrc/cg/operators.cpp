@@ -131,6 +131,7 @@ class Writer {
     tensors_ << "tensor " << name << " " << elem << " " << role << " " << rank << " " << dims << "\n";
     types_[name] = std::make_pair(ElemType(elem), std::string(role) == "in");
   }
+  bool Has(const std::string& tensor) const { return types_.count(tensor) != 0; }
   void Scalar(const std::string& name) { scalars_ << "scalar " << name << " f32\n"; }
   void Header(const std::string& h) { headers_ << "#include \"" << h << "\"\n"; }
   void Comment(const std::string& c) { body_ << "// " << c << "\n"; }
@@ -366,10 +367,12 @@ struct Product {
   std::string epi;                    // an expression of the epilogue's type
 };
 
-// Rows of a forward product that product_few takes, and its split of k: at
-// least kFewK of it for each workgroup that shares a strip, and no more
-// workgroups than kFewBlocks.
-constexpr uint32_t kFewRows = 64, kFewK = 256, kFewBlocks = 256;
+// Rows of a forward product that product_few takes.
+constexpr uint32_t kFewRows = 64;
+// Workgroups that products of few tiles are split into, by k: as many as CUs.
+constexpr uint32_t kCUs = 256;
+// Planes of at most so many results may be split (128 tiles of 128x128).
+constexpr uint64_t kSplitPlane = 1ull << 21;
 
 void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   std::ostringstream ops;
@@ -380,82 +383,136 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
       ops << "  p.b[" << h << "][" << s << "] = reinterpret_cast<const uint16_t*>(" << p.B[p.pair ? h : 0][s] << ");\n";
   }
   ops << "  p.M = " << p.M << ";\n  p.N = " << p.N << ";\n  p.K = " << p.K << ";\n  const auto epi = " << p.epi << ";\n";
-  const std::string f16 = Bool(a.elem == "f16");
-  const std::string targs = f16 + ", " + Bool(p.a_rc) + ", " + Bool(p.b_rc) + ", " + Bool(p.pair) + ", " + std::to_string(p.segs);
-  auto body = [&](const std::string& call) { return ops.str() + "  tca::hip::" + call + "(p, epi, blockIdx.x);\n"; };
+  const std::string f16 = Bool(a.elem == "f16"), pair = Bool(p.pair);
+  const std::string targs = f16 + ", " + Bool(p.a_rc) + ", " + Bool(p.b_rc) + ", " + pair + ", " + std::to_string(p.segs);
+  const std::string plane = p.M + "*" + p.N, part = "part";
+  // Tiles of rows x cols (of a pair: cols / 2 of each product) as grid terms, and counted on the device.
   auto tiles = [&](uint32_t rows, uint32_t cols) {
     return p.M + "/" + std::to_string(rows) + " " + p.N + "/" + std::to_string(p.pair ? cols / 2u : cols);
   };
+  auto count = [&](uint32_t rows, uint32_t cols) {
+    const std::string r = std::to_string(rows) + "u", c = std::to_string(p.pair ? cols / 2u : cols) + "u";
+    return "((p.M - 1u) / " + r + " + 1u) * ((p.N - 1u) / " + c + " + 1u)";
+  };
+  // k in P parts, at least `least` of it in each, where `terms` make fewer than kCUs workgroups.
+  auto split = [&](uint32_t least, const std::string& terms, const char* mode) {
+    int n = 0;
+    std::istringstream in(terms);
+    for (std::string t; in >> t;) ++n;
+    return "split " + p.K + " " + std::to_string(least) + " " + std::to_string(kCUs) + " " + mode + " " + std::to_string(n) + " " + terms;
+  };
+  auto parts = [&](uint32_t least, const std::string& blocks) {
+    return "tca::hip::col_split(p.K, " + blocks + ", " + std::to_string(least) + "u, " + std::to_string(kCUs) + "u)";
+  };
+  auto join = [&](const std::string& suffix, const std::string& P, const std::string& record, std::vector<std::string> records,
+                  const std::string& of) {
+    Writer::Kernel j;
+    j.suffix = p.suffix + suffix;
+    j.params = p.params + " " + part;
+    j.block = 128;
+    j.body = ops.str() + "  tca::hip::join_parts<" + pair + ">(" + part + ", epi, p.M, p.N, " + P + ");\n";
+    j.grid = p.M + "/1 " + p.N + "/1024";
+    j.records = std::move(records);
+    j.records.push_back(record);
+    j.detail = p.what + ", the partial sums of " + of + " (P > 1 only)";
+    w->Add(j);
+  };
+  // The partial sums of kCUs workgroups, of 128x128 results each at most (of few
+  // rows 64x64, of a pair twice that): products of one program run in turn and share it.
+  if (!w->Has(part)) {
+    w->Dim("part_dim", uint64_t{kCUs} * 128u * 128u);
+    w->Tensor(part, "f32", "local", "part_dim");
+  }
+
   // A forward product of few rows, at any alignment.
   const bool few = !p.a_rc && p.b_rc;
   if (few) {
-    const std::string strips = "((N - 1u) / tca::hip::kFewColumns + 1u)";
-    const std::string P = "tca::hip::col_split(K, " + strips + ", " + std::to_string(kFewK) + "u, " + std::to_string(kFewBlocks) + "u)";
-    const std::string split = "split K " + std::to_string(kFewK) + " " + std::to_string(kFewBlocks) + " ";
-    w->Dim("few_parts", uint64_t{kFewBlocks} * 64u * kFewRows * (p.pair ? 2u : 1u));
-    w->Tensor("few_part", "f32", "local", "few_parts");
+    const uint32_t least = 256;  // a step for each wave
+    const std::string strips = "((p.N - 1u) / tca::hip::kFewColumns + 1u)", P = parts(least, strips), terms = p.N + "/64";
     uint32_t from = 1;
     for (uint32_t blocks : {1u, 2u, 4u}) {
       Writer::Kernel k;
       k.suffix = p.suffix + "_few" + std::to_string(16u * blocks);
-      k.params = p.params + " few_part";
+      k.params = p.params + " " + part;
       k.block = 512;
-      k.body = ops.str() + "  tca::hip::product_few<" + f16 + ", " + Bool(p.pair) + ", " + std::to_string(blocks) + ">(p, epi, few_part, " +
+      k.body = ops.str() + "  tca::hip::product_few<" + f16 + ", " + pair + ", " + std::to_string(blocks) + ">(p, epi, " + part + ", " +
                strips + ", " + P + ");\n";
-      k.grid = "N/64";
-      k.records = {split + "0 1 N/64", When("M", from, 16u * blocks)};
+      k.grid = terms;
+      k.records = {split(least, terms, "0"), When("M", from, 16u * blocks)};
       k.detail = p.what + ", " + std::to_string(from) + " to " + std::to_string(16u * blocks) + " rows, strips of 64 columns, k over 8 waves and P workgroups";
       w->Add(k);
       from = 16u * blocks + 1u;
     }
-    Writer::Kernel j;
-    j.suffix = p.suffix + "_fewjoin";
-    j.params = p.params + " few_part";
-    j.body = ops.str() + "  tca::hip::few_join<" + Bool(p.pair) + ">(few_part, epi, M, N, " + P + ");\n";
-    j.grid = "M/1 N/2048";
-    j.records = {split + "1 1 N/64", When("M", 1, kFewRows)};
-    j.detail = p.what + ", the partial sums of few rows (P > 1 only)";
-    w->Add(j);
+    join("_fewjoin", P, split(least, terms, "1"), {When("M", 1, kFewRows)}, "few rows");
   }
-  const std::string many = When("M", kFewRows + 1u, kMost);
   // Rows of whole 16-byte chunks, of both operands, go straight into LDS.
   std::vector<std::string> aligned, odd;
   for (const std::string& d : std::set<std::string>{p.a_rc ? p.M : p.K, p.b_rc ? p.N : p.K}) {
     aligned.push_back(When(d, 0, kMost, 8));
     odd.push_back("unless " + d + " 0 " + std::to_string(kMost) + " 8 0");
   }
-  if (few) aligned.push_back(many);
-  if (few) odd.push_back(many);
+  if (few) aligned.push_back(When("M", kFewRows + 1u, kMost));
+  if (few) odd.push_back(When("M", kFewRows + 1u, kMost));
+  const std::string small_plane = When(plane, 0, kSplitPlane), large_plane = When(plane, kSplitPlane + 1u, 18446744073709551615ull);
+  auto with = [](std::vector<std::string> v, std::initializer_list<std::string> r) {
+    v.insert(v.end(), r);
+    return v;
+  };
+  const std::string whole = "(p, epi, blockIdx.x, 0u, (p.K + 63u) / 64u * " + std::to_string(p.segs) + "u);\n";
+  auto body = [&](const std::string& call) { return ops.str() + "  tca::hip::" + call + whole; };
+  // One product of few tiles: `call` on the tile and chunk of k of a workgroup.
+  auto few_tiles = [&](const std::string& suffix, const std::string& call, uint32_t block, uint32_t rows, const std::vector<std::string>& records,
+                       const std::string& detail) {
+    const uint32_t least = 512;  // eight turns
+    const std::string P = parts(least, count(rows, 128)), terms = tiles(rows, 128);
+    Writer::Kernel k;
+    k.suffix = p.suffix + suffix;
+    k.params = p.params + " " + part;
+    k.block = block;
+    k.body = ops.str() + "  const uint32_t tiles = " + count(rows, 128) + ", P = " + P + ";\n" +
+             "  const uint32_t chunk = blockIdx.x / tiles;\n  const tca::hip::Run run = tca::hip::run_of(p.K, " +
+             std::to_string(p.segs) + "u, chunk, P);\n  tca::hip::" + call + "(p, tca::hip::split_store<" + pair + ">(epi, " + part +
+             ", chunk, P, p.M, p.N), blockIdx.x % tiles, run.first, run.end);\n";
+    k.grid = terms;
+    k.records = with(records, {split(least, terms, "0"), small_plane});
+    k.detail = p.what + ", " + detail + ", k over P workgroups (at most " + std::to_string(kSplitPlane) + " results)";
+    w->Add(k);
+    join(suffix + "join", P, split(least, terms, "1"), with(records, {small_plane}), detail);
+  };
+  few_tiles("_k", "product_ring<" + targs + ", 128, 64, 2, 2, 5, 5>", 256, 128, aligned, "tiles of 128x128, direct to LDS");
   Writer::Kernel k;
   k.suffix = p.suffix + "_r";
   k.params = p.params;
-  k.records = aligned;
+  k.records = with(aligned, {large_plane});
   k.body = body("product_ring<" + targs + ", 128, 64, 2, 2, 5, 5>");
   k.grid = tiles(128, 128);
   k.detail = p.what + ", tiles of 128x128 (256x256, 256x128 where they fill the card), 4 waves, direct to LDS";
-  auto form = [&](const char* suffix, const std::string& what, const std::string& config, uint32_t rows, uint32_t cols,
-                  uint32_t most, const std::string& of) {
-    const std::string grid = tiles(rows, cols);
-    // its grid, then the bound: at least `most` tiles, of `of`
-    k.forms.push_back({p.suffix + suffix, body("product_ring<" + targs + ", " + config + ">"), p.what + ", " + what,
-                       "0 2 1 2 " + grid + " " + std::to_string(most) + " 2 " + of});
+  auto form = [&](Writer::Kernel* of, const char* suffix, const std::string& what, const std::string& call, uint32_t rows,
+                  uint32_t cols, uint32_t least, const std::string& terms) {
+    // its grid, then the bound: at least so many tiles, of `terms`
+    of->forms.push_back({p.suffix + suffix, body(call), p.what + ", " + what,
+                         "0 2 1 2 " + tiles(rows, cols) + " " + std::to_string(least) + " 2 " + terms});
   };
   const std::string large = tiles(256, 256), tall = tiles(256, 128), small = tiles(128, 128);
   const std::string what_l = "tiles of 256x256", what_m = "tiles of 256x128", what_s = "tiles of 128x128, two workgroups a CU";
-  const std::string cfg_l = "256, 128, 2, 2, 3, 2", cfg_m = "256, 64, 2, 2, 3, 3", cfg_s = "128, 64, 2, 2, 3, 2";
-  form("_l", what_l, cfg_l, 256, 256, 385, large);
-  form("_m", what_m, cfg_m, 256, 128, 257, large);
-  form("_l", what_l, cfg_l, 256, 256, 192, large);
-  form("_m", what_m, cfg_m, 256, 128, 192, tall);
-  form("_s", what_s, cfg_s, 128, 128, 257, small);
+  const std::string ring = "product_ring<" + targs;
+  const std::string cfg_l = ring + ", 256, 128, 2, 2, 3, 2>", cfg_m = ring + ", 256, 64, 2, 2, 3, 3>", cfg_s = ring + ", 128, 64, 2, 2, 3, 2>";
+  form(&k, "_l", what_l, cfg_l, 256, 256, 385, large);
+  form(&k, "_m", what_m, cfg_m, 256, 128, 257, large);
+  form(&k, "_l", what_l, cfg_l, 256, 256, 192, large);
+  form(&k, "_m", what_m, cfg_m, 256, 128, 192, tall);
+  form(&k, "_s", what_s, cfg_s, 128, 128, 257, small);
   w->Add(k);
+  few_tiles("_o", "product_any<" + targs + ", 64>", 512, 64, odd, "tiles of 64x128, any shape and alignment");
   Writer::Kernel any;
   any.suffix = p.suffix;
   any.params = p.params;
-  any.records = odd;
-  any.body = body("product_any<" + targs + ">");
-  any.grid = tiles(128, 128);
-  any.detail = p.what + ", tiles of 128x128, any shape and alignment";
+  any.block = 512;
+  any.records = with(odd, {large_plane});
+  any.body = body("product_any<" + targs + ", 64>");
+  any.grid = tiles(64, 128);
+  any.detail = p.what + ", tiles of 64x128 (128x128 where they fill the card), any shape and alignment";
+  form(&any, "_a", "tiles of 128x128, any shape and alignment", "product_any<" + targs + ", 128>", 128, 128, kCUs, small);
   w->Add(any);
 }
 

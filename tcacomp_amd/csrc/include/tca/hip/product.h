@@ -182,21 +182,53 @@ struct PlainStore {
   }
 };
 
+// The epilogue of a product whose k is split over P workgroups: P == 1 the
+// product's own, otherwise the partial sums of chunk c as rows of f32
+// (`part` is [P][1 or 2][M][N]; join_parts adds them in order).
+template <typename Epi>
+struct SplitStore {
+  const Epi& epi;
+  PlainStore<float> part;
+  bool direct;
+  using Fetch = typename Epi::Fetch;
+  template <bool WHOLE>
+  __device__ __forceinline__ Fetch fetch(uint32_t m, uint32_t n) const {
+    return direct ? epi.template fetch<WHOLE>(m, n) : Fetch{};
+  }
+  template <bool WHOLE, typename... V>
+  __device__ __forceinline__ void store(uint32_t m, uint32_t n, const Fetch& f, V&... v) const {
+    if (direct) epi.template store<WHOLE>(m, n, f, v...);
+    else part.template store<WHOLE>(m, n, NoFetch{}, v...);
+  }
+};
+template <bool PAIR, typename Epi>
+__device__ __forceinline__ SplitStore<Epi> split_store(const Epi& epi, float* part, uint32_t chunk, uint32_t P, uint32_t M, uint32_t N) {
+  const uint64_t plane = static_cast<uint64_t>(M) * N;
+  float* at = part + chunk * (PAIR ? 2u : 1u) * plane;
+  return SplitStore<Epi>{epi, PlainStore<float>{at, at + plane, N}, P == 1u};
+}
+
 // A wave's results to the epilogue: IM blocks of 16 rows by JH blocks of 16
-// columns of either half (acc[i][j], j < JH the first half), 64 rows at a time
-// through `lds` (64 x 32 JH floats of the wave's own), so that a lane takes
-// eight consecutive columns, the memory accesses of a row are whole lines, and
-// the epilogue's code is there once and not once for each block. 16-byte slot
-// c of row r lies at c ^ (r % 16): the writes of a block's 16 rows cover the
-// banks once. Four chunks a turn, the next turn's loads issued before this
+// columns of either half (acc[i][j], j < JH the first half), at most 64 rows at a
+// time through `lds` (those rows by 32 JH floats, the wave's own), so that a lane
+// takes eight consecutive columns, the memory accesses of a row are whole
+// lines, and the epilogue's code is there once and not once for each block.
+// 16-byte slot c of row r lies at c ^ store_swizzle(r): the writes of a
+// block's 16 rows cover the banks once. Four chunks a turn, the next turn's loads issued before this
 // one's stores: a wave has its SIMD to itself, nothing else covers their
 // latency. WHOLE: every chunk lies inside the plane.
+template <uint32_t SLOTS>
+__device__ __forceinline__ uint32_t store_swizzle(uint32_t r) {
+  return SLOTS >= 16u ? r & 15u : (r >> 1) & 7u;  // rows of 128 bytes: two to the banks
+}
 template <int IM, int JH, bool PAIR, bool WHOLE, typename Epi>
 __device__ __forceinline__ void product_store(const f32x4_t (&acc)[IM][2 * JH], float* lds, uint32_t m0, uint32_t n0,
                                               uint32_t half, uint32_t M, uint32_t N, const Epi& epi, uint32_t lane) {
   constexpr uint32_t TH = 16u * JH, PITCH = 2u * TH, CHUNKS = PAIR ? TH / 8u : TH / 4u;  // of a row
-  constexpr uint32_t TURN = 4, TURNS = CHUNKS / TURN, PASSES = IM / 4;
-  static_assert(IM % 4 == 0 && CHUNKS % TURN == 0, "64 rows at a time, whole turns");
+  constexpr int IP = IM < 4 ? IM : 4;  // blocks of rows at a time
+  constexpr uint32_t ROWS = 16u * IP, COUNT = ROWS * CHUNKS / 64u, TURN = COUNT < 4u ? COUNT : 4u, TURNS = COUNT / TURN;
+  constexpr uint32_t PASSES = IM / IP, SLOTS = PITCH / 4u;
+  static_assert(IM % IP == 0 && ROWS * CHUNKS % 64u == 0u && COUNT % TURN == 0u && SLOTS >= 8u, "whole turns");
   typename Epi::Fetch now[TURN], next[TURN];
   auto row_of = [&](uint32_t t) { return (t * 64u + lane) / CHUNKS; };  // of a pass
   auto col_of = [&](uint32_t t) { return (t * 64u + lane) % CHUNKS; };
@@ -204,7 +236,7 @@ __device__ __forceinline__ void product_store(const f32x4_t (&acc)[IM][2 * JH], 
 #pragma unroll
     for (uint32_t i = 0; i < TURN; ++i) {
       const uint32_t t = turn % TURNS * TURN + i, k = col_of(t);
-      const uint32_t m = m0 + 64u * (turn / TURNS) + row_of(t), n = n0 + k / (TH / 8u) * half + k % (TH / 8u) * 8u;
+      const uint32_t m = m0 + ROWS * (turn / TURNS) + row_of(t), n = n0 + k / (TH / 8u) * half + k % (TH / 8u) * 8u;
       if (WHOLE || (m < M && n < N)) f[i] = epi.template fetch<WHOLE>(m, n);
     }
   };
@@ -216,11 +248,11 @@ __device__ __forceinline__ void product_store(const f32x4_t (&acc)[IM][2 * JH], 
     for (int p = 0; p < static_cast<int>(PASSES); ++p) {
       if (pass != static_cast<uint32_t>(p)) continue;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < IP; ++i)
 #pragma unroll
         for (int j = 0; j < 2 * JH; ++j) {
           const uint32_t r = 16u * i + (lane & 15u), c = 4u * j + (lane >> 4);
-          *reinterpret_cast<f32x4_t*>(&lds[r * PITCH + ((c ^ (r & 15u)) << 2)]) = acc[4 * p + i][j];
+          *reinterpret_cast<f32x4_t*>(&lds[r * PITCH + ((c ^ store_swizzle<SLOTS>(r)) << 2)]) = acc[IP * p + i][j];
         }
     }
     wave_exchange();
@@ -231,11 +263,11 @@ __device__ __forceinline__ void product_store(const f32x4_t (&acc)[IM][2 * JH], 
 #pragma unroll
       for (uint32_t i = 0; i < TURN; ++i) {
         const uint32_t t = b * TURN + i, r = row_of(t), k = col_of(t), h = k / (TH / 8u), c = h * (TH / 4u) + k % (TH / 8u) * 2u;
-        const uint32_t m = m0 + 64u * pass + r, n = n0 + h * half + k % (TH / 8u) * 8u;
+        const uint32_t m = m0 + ROWS * pass + r, n = n0 + h * half + k % (TH / 8u) * 8u;
         const float* row = &lds[r * PITCH];
         auto take = [&](uint32_t s, float (&v)[8]) {
-          const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(&row[(s ^ (r & 15u)) << 2]);
-          const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(&row[((s + 1u) ^ (r & 15u)) << 2]);
+          const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(&row[(s ^ store_swizzle<SLOTS>(r)) << 2]);
+          const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(&row[((s + 1u) ^ store_swizzle<SLOTS>(r)) << 2]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             v[e] = lo[e];
@@ -279,28 +311,30 @@ __device__ __forceinline__ u32x4 gather16(const uint16_t* p, uint32_t n) {
                static_cast<uint32_t>(hi >> 32)};
 }
 
-// ------------------------------------- any shape, any alignment: 128x128 tiles
-// 4 waves of 64x64 (of a pair: 64x32 of each product), 64-deep slices of K,
-// global memory -> registers (16 bytes a lane, unguarded: rows and chunks past
-// the end re-read the last ones) -> LDS (two buffers, one barrier a slice).
-// A chunk that runs past the end of its row is loaded from 8 elements before
-// that end and moved into place, so the tail of k adds zeros.
-template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, typename Epi>
-__device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& epi, uint32_t tile) {
-  constexpr uint32_t BM = 128, HB = 64, SLICE = BM * 64u, HALF = HB * 64u, BUF = SLICE + 2u * HALF;
+// ------------------------------------- any shape, any alignment
+// Tiles of BM x 128 (a pair: BM x 64 of each product), 8 waves, 2 x 4 of them,
+// 64-deep slices of K: global memory -> registers (16 bytes a lane, two slices
+// ahead, unguarded: rows and chunks past the end re-read the last ones) -> LDS
+// (two buffers, one barrier a slice). A chunk that runs past the end of its row
+// is loaded from 8 elements before that end and moved into place, so the tail
+// of k adds zeros. Slices first .. end - 1 of all segments'.
+template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, typename Epi>
+__device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& epi, uint32_t tile, uint32_t first, uint32_t end) {
+  constexpr uint32_t HB = 64, THREADS = 512, SLICE = BM * 64u, HALF = HB * 64u, BUF = SLICE + 2u * HALF;
+  constexpr int IM = BM / 32, CA = BM * 8 / THREADS;
   __shared__ __attribute__((aligned(16))) uint16_t lds[2 * BUF];
   const uint32_t M = p.M, N = p.N, K = p.K, width = PAIR ? HB : 2u * HB;
   uint32_t tm, tn;
   gemm_tile_coords((M - 1u) / BM + 1u, (N - 1u) / width + 1u, &tm, &tn, tile);
   const uint32_t m0 = tm * BM, n0 = tn * width;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t wm = (wave >> 1) * 64u, wn = (wave & 1u) * 32u;
+  const uint32_t wm = (wave >> 2) * (BM / 2u), wn = (wave & 3u) * 16u;
 
   // One chunk of 8 of a K-contiguous panel row, or of row k of a row-contiguous
-  // panel of W columns, and its place in a slice.
+  // panel, and its values in place.
   auto kc_load = [&](const uint16_t* base, uint32_t row, uint32_t rows, uint32_t k) -> u32x4 {
     const uint16_t* r = base + static_cast<uint64_t>(row < rows ? row : rows - 1u) * K;
-    if (K < 8u) return gather16(r + k, k < K ? K - k : 0u);
+    if (K < 8u) return gather16(r + (k < K ? k : 0u), k < K ? K - k : 0u);
     return load16_any(r + (k < K - 8u ? k : K - 8u));
   };
   auto kc_fix = [&](u32x4 v, uint32_t k) -> u32x4 {
@@ -315,104 +349,117 @@ __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& 
     if (k >= K) return u32x4{0u, 0u, 0u, 0u};
     return cols < 8u || c + 8u <= cols ? v : shift_down16(v, c - (cols - 8u));
   };
-  u32x4 ra[4], rb[2][2];
-  const uint32_t ns = (K + 63u) / 64u, total = ns * SEGS;
-  auto load = [&](uint32_t t) {
+  // A panel of W columns has W / 8 chunks a row of k; HB = 64: 8, as a row of k has.
+  constexpr uint32_t kAC = A_RC ? BM / 8u : 8u;
+  struct Regs {
+    u32x4 a[CA], b[2];
+  };
+  Regs regs[2];
+  const uint32_t ns = (K + 63u) / 64u;
+  auto load = [&](Regs& r, uint32_t t) {
     const uint32_t seg = SEGS == 1 || t < ns ? 0u : 1u, k0 = (t - seg * ns) * 64u;
-    const uint16_t* a = SEGS == 1 || seg == 0u ? p.a[0] : p.a[SEGS - 1];
+    const uint16_t* a = seg == 0u ? p.a[0] : p.a[SEGS - 1];
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) {
-      const uint32_t c = i * 256u + tid;
-      ra[i] = A_RC ? rc_load(a, m0 + (c & 15u) * 8u, M, k0 + (c >> 4)) : kc_load(a, m0 + (c >> 3), M, k0 + (c & 7u) * 8u);
+    for (uint32_t i = 0; i < CA; ++i) {
+      const uint32_t c = i * THREADS + tid;
+      r.a[i] = A_RC ? rc_load(a, m0 + c % kAC * 8u, M, k0 + c / kAC) : kc_load(a, m0 + (c >> 3), M, k0 + (c & 7u) * 8u);
     }
 #pragma unroll
     for (uint32_t h = 0; h < 2u; ++h) {
       const uint32_t hp = PAIR ? h : 0u, nh = PAIR ? n0 : n0 + HB * h;
-      const uint16_t* b = SEGS == 1 || seg == 0u ? p.b[hp][0] : p.b[hp][SEGS - 1];
-#pragma unroll
-      for (uint32_t i = 0; i < 2u; ++i) {
-        const uint32_t c = i * 256u + tid;
-        rb[h][i] = B_RC ? rc_load(b, nh + (c & 7u) * 8u, N, k0 + (c >> 3)) : kc_load(b, nh + (c >> 3), N, k0 + (c & 7u) * 8u);
-      }
+      const uint16_t* b = seg == 0u ? p.b[hp][0] : p.b[hp][SEGS - 1];
+      r.b[h] = B_RC ? rc_load(b, nh + (tid & 7u) * 8u, N, k0 + (tid >> 3)) : kc_load(b, nh + (tid >> 3), N, k0 + (tid & 7u) * 8u);
     }
   };
-  auto write = [&](uint32_t t) {
+  auto write = [&](Regs& r, uint32_t t, uint32_t buf) {
     const uint32_t k0 = (SEGS == 1 || t < ns ? t : t - ns) * 64u;
-    uint16_t* As = lds + (t & 1u) * BUF;
+    uint16_t* As = lds + buf * BUF;
     const bool ktail = k0 + 64u > K;
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) {
-      const uint32_t c = i * 256u + tid;
+    for (uint32_t i = 0; i < CA; ++i) {
+      const uint32_t c = i * THREADS + tid;
       if constexpr (A_RC) {
-        const uint32_t k = c >> 4, m = (c & 15u) * 8u;
-        if (ktail || m0 + BM > M) ra[i] = rc_fix(ra[i], m0 + m, M, k0 + k);
-        *reinterpret_cast<u32x4*>(&As[swz_kn<BM>(k, m)]) = ra[i];
+        const uint32_t k = c / kAC, m = c % kAC * 8u;
+        if (ktail || m0 + BM > M) r.a[i] = rc_fix(r.a[i], m0 + m, M, k0 + k);
+        *reinterpret_cast<u32x4*>(&As[swz_kn<BM>(k, m)]) = r.a[i];
       } else {
-        if (ktail) ra[i] = kc_fix(ra[i], k0 + (c & 7u) * 8u);
-        *reinterpret_cast<u32x4*>(&As[swz_rows64(c >> 3, c & 7u)]) = ra[i];
+        if (ktail) r.a[i] = kc_fix(r.a[i], k0 + (c & 7u) * 8u);
+        *reinterpret_cast<u32x4*>(&As[swz_rows64(c >> 3, c & 7u)]) = r.a[i];
       }
     }
 #pragma unroll
     for (uint32_t h = 0; h < 2u; ++h) {
       uint16_t* Bs = As + SLICE + h * HALF;
       const uint32_t nh = PAIR ? n0 : n0 + HB * h;
-#pragma unroll
-      for (uint32_t i = 0; i < 2u; ++i) {
-        const uint32_t c = i * 256u + tid;
-        if constexpr (B_RC) {
-          const uint32_t k = c >> 3, n = (c & 7u) * 8u;
-          if (ktail || nh + HB > N) rb[h][i] = rc_fix(rb[h][i], nh + n, N, k0 + k);
-          *reinterpret_cast<u32x4*>(&Bs[swz_kn<HB>(k, n)]) = rb[h][i];
-        } else {
-          if (ktail) rb[h][i] = kc_fix(rb[h][i], k0 + (c & 7u) * 8u);
-          *reinterpret_cast<u32x4*>(&Bs[swz_rows64(c >> 3, c & 7u)]) = rb[h][i];
-        }
+      if constexpr (B_RC) {
+        const uint32_t k = tid >> 3, n = (tid & 7u) * 8u;
+        if (ktail || nh + HB > N) r.b[h] = rc_fix(r.b[h], nh + n, N, k0 + k);
+        *reinterpret_cast<u32x4*>(&Bs[swz_kn<HB>(k, n)]) = r.b[h];
+      } else {
+        if (ktail) r.b[h] = kc_fix(r.b[h], k0 + (tid & 7u) * 8u);
+        *reinterpret_cast<u32x4*>(&Bs[swz_rows64(tid >> 3, tid & 7u)]) = r.b[h];
       }
     }
   };
-  f32x4_t acc[4][4];  // [block of rows][2 h + block of columns]
+  f32x4_t acc[IM][2];  // [block of rows][half]
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < IM; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  auto compute = [&](uint32_t t) {
-    const uint16_t* As = lds + (t & 1u) * BUF;
+    for (int h = 0; h < 2; ++h) acc[i][h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  auto compute = [&](uint32_t buf) {
+    const uint16_t* As = lds + buf * BUF;
 #pragma unroll
     for (uint32_t s = 0; s < 2u; ++s) {
-      bf16x8 fa[4];
+      bf16x8 fa[IM], fb[2];
 #pragma unroll
-      for (uint32_t i = 0; i < 4u; ++i) {
+      for (uint32_t i = 0; i < IM; ++i) {
         if constexpr (A_RC) fa[i] = frag_b16_tr<BM>(As, wm + 16u * i, lane, 32u * s);
         else fa[i] = *reinterpret_cast<const bf16x8*>(&As[swz_rows64(wm + 16u * i + (lane & 15u), 4u * s + (lane >> 4))]);
       }
 #pragma unroll
       for (uint32_t h = 0; h < 2u; ++h) {
         const uint16_t* Bs = As + SLICE + h * HALF;
+        if constexpr (B_RC) fb[h] = frag_b16_tr<HB>(Bs, wn, lane, 32u * s);
+        else fb[h] = *reinterpret_cast<const bf16x8*>(&Bs[swz_rows64(wn + (lane & 15u), 4u * s + (lane >> 4))]);
+      }
+      // Operands swapped: a lane ends with four consecutive columns of one row.
 #pragma unroll
-        for (uint32_t j = 0; j < 2u; ++j) {
-          bf16x8 fb;
-          if constexpr (B_RC) fb = frag_b16_tr<HB>(Bs, wn + 16u * j, lane, 32u * s);
-          else fb = *reinterpret_cast<const bf16x8*>(&Bs[swz_rows64(wn + 16u * j + (lane & 15u), 4u * s + (lane >> 4))]);
-          // Operands swapped: a lane ends with four consecutive columns of one row.
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (uint32_t i = 0; i < 4u; ++i) acc[i][2u * h + j] = mfma_16x16x32_16b<F16>(fb, fa[i], acc[i][2u * h + j]);
+        for (int i = 0; i < IM; ++i) acc[i][h] = mfma_16x16x32_16b<F16>(fb[h], fa[i], acc[i][h]);
+    }
+  };
+  if (first < end) {
+    load(regs[0], first);
+    if (first + 1u < end) load(regs[1], first + 1u);
+    write(regs[0], first, 0u);
+    if (first + 2u < end) load(regs[0], first + 2u);
+    __syncthreads();
+    for (uint32_t t = first; t < end; t += 2u) {
+#pragma unroll
+      for (uint32_t i = 0; i < 2u; ++i) {  // slice t + i, in buffer i; the next one in the registers of its parity
+        const uint32_t s = t + i;
+        if (s < end) {
+          compute(i);
+          if (s + 1u < end) write(regs[1u - i], s + 1u, 1u - i);
+          if (s + 3u < end) load(regs[1u - i], s + 3u);
+          __syncthreads();
         }
       }
     }
-  };
-  if (total > 0u) {
-    load(0u);
-    write(0u);
-    __syncthreads();
-    for (uint32_t t = 0; t < total; ++t) {
-      if (t + 1u < total) load(t + 1u);
-      compute(t);
-      if (t + 1u < total) write(t + 1u);
-      __syncthreads();
-    }
   }
   // (the last slice's barrier: no wave reads the slices any more)
-  product_store<4, 2, PAIR, false>(acc, reinterpret_cast<float*>(lds) + wave * (64u * 64u), m0 + wm, n0 + wn, HB, M, N, epi, lane);
+  product_store<IM, 1, PAIR, false>(acc, reinterpret_cast<float*>(lds) + wave * (32u * (IM < 4 ? 16u * IM : 64u)), m0 + wm, n0 + wn, HB, M, N,
+                                    epi, lane);
+}
+
+// The 64-deep slices of all segments' that chunk c of P takes: a run of them.
+struct Run {
+  uint32_t first, end;
+};
+__device__ __forceinline__ Run run_of(uint32_t K, uint32_t segs, uint32_t chunk, uint32_t P) {
+  const uint32_t total = (K + 63u) / 64u * segs, per = (total + P - 1u) / P, first = chunk * per;
+  return Run{first < total ? first : total, first + per < total ? first + per : total};
 }
 
 // ------------------------- rows of whole 16-byte chunks: straight into LDS
@@ -523,7 +570,7 @@ constexpr int loads_after(int at, int qa, int qb) {
 // Every turn issues the same loads: a chunk outside its operand, or past the
 // last turn, is read from kZeroChunk, so no tail of k, edge of the plane or
 // border between segments needs code of its own, and the count of loads in
-// flight is static. (The operands are __restrict__ parameters: without them
+// flight is static. Turns first .. end - 1 of all segments'. (The operands are __restrict__ parameters: without them
 // the compiler takes a transposing read of LDS to depend on every load into it
 // and waits for all of them.)
 template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, uint32_t HB, uint32_t WGM, uint32_t WGN, int SA, int SB,
@@ -532,7 +579,7 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
                                                 const uint16_t* __restrict__ pb00, const uint16_t* __restrict__ pb01,
                                                 const uint16_t* __restrict__ pb10, const uint16_t* __restrict__ pb11,
                                                 const uint16_t* __restrict__ zero, uint32_t M, uint32_t N, uint32_t K,
-                                                const Epi& epi, uint32_t tile) {
+                                                const Epi& epi, uint32_t tile, uint32_t first, uint32_t end) {
   constexpr uint32_t WAVES = WGM * WGN, TM = BM / WGM, TH = HB / WGN, ASL = BM * 64u, BSL = HB * 64u;
   constexpr int IM = TM / 16, JH = TH / 16, JN = 2 * JH, QA = BM / 8 / WAVES, QB = 2 * HB / 8 / WAVES;
   static_assert(BM / 8 % WAVES == 0 && HB / 8 % WAVES == 0, "whole chunks, of either half, per wave");
@@ -547,15 +594,15 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
   const uint32_t pitch_a = A_RC ? M : K, pitch_b = B_RC ? N : K;
   const Fill<A_RC, BM, WAVES> fill_a(wave, lane, pitch_a);
   const Fill<B_RC, HB, WAVES> fill_b(wave, lane, pitch_b);
-  const uint32_t ns = (K + 63u) / 64u, total = ns * SEGS;
+  const uint32_t ns = (K + 63u) / 64u;
   uint16_t* ldsp = lds;
   // Turns whose chunks all lie inside the operands, for a tile that does:
   // their loads take the panel's address from scalar registers and a 32-bit
   // offset a lane, with no test (which costs a tenth of the whole time).
   const bool inner = m0 + BM <= M && n0 + width <= N && M <= kInnerMost && N <= kInnerMost && K <= kInnerMost;
-  const uint32_t whole = !inner ? 0u : K % 64u == 0u ? total : SEGS == 1 ? K / 64u : 0u;
+  const uint32_t full = K % 64u == 0u ? end : SEGS == 1 ? K / 64u : 0u, whole = !inner ? 0u : full < end ? full : end;
   // The first k of turn t in its segment; past the last turn every chunk is zeros.
-  auto first_k = [&](uint32_t t) { return t < total ? (SEGS == 1 || t < ns ? t : t - ns) * 64u : K; };
+  auto first_k = [&](uint32_t t) { return t < end ? (SEGS == 1 || t < ns ? t : t - ns) * 64u : K; };
   auto load_a = [&](auto fast, uint32_t t, uint32_t slot, int q) {
     const uint32_t k0 = first_k(t);
     const uint16_t* p = (SEGS == 1 || t < ns ? pa0 : pa1) +
@@ -643,10 +690,10 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
   for (int t = 0; t < (SA - 1 > SB ? SA - 1 : SB); ++t) {
     if (t < SA - 1)
 #pragma unroll
-      for (int q = 0; q < QA; ++q) load_a(Checked{}, t, t * kA, q);
+      for (int q = 0; q < QA; ++q) load_a(Checked{}, first + t, t * kA, q);
     if (t < SB)
 #pragma unroll
-      for (int q = 0; q < QB; ++q) load_b(Checked{}, t, kB0 + t * kB, q);
+      for (int q = 0; q < QB; ++q) load_b(Checked{}, first + t, kB0 + t * kB, q);
   }
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(waitcnt_imm(kStart - QA - QB, 0));
@@ -656,13 +703,13 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
   for (int i = 0; i < IM; ++i) a0[i] = rd_a(a_this, 0, i);
 #pragma unroll
   for (int j = 0; j < JN; ++j) b0[j] = rd_b(b_this, 0, j);
-  // K = 0 is one turn of zeros (a branch round the loop would hold the
-  // accumulators in two places, and spill).
-  uint32_t t = 0u;
+  // No turns at all (K = 0) is one of zeros: a branch round the loop would hold
+  // the accumulators in two places, and spill.
+  uint32_t t = first;
   constexpr uint32_t kAhead = SA - 1 > SB ? SA - 1 : SB;
   for (; t + kAhead < whole; ++t) turn(Fast{}, t);
   do turn(Checked{}, t++);
-  while (t < total);
+  while (t < end);
   // No load into LDS is in flight past the loop, in any wave.
   __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
   __builtin_amdgcn_s_barrier();
@@ -678,10 +725,10 @@ __device__ __forceinline__ void product_ring_of(const uint16_t* __restrict__ pa0
 
 template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, uint32_t HB, uint32_t WGM, uint32_t WGN, int SA, int SB,
           typename Epi>
-__device__ __forceinline__ void product_ring(const Operands<SEGS>& p, const Epi& epi, uint32_t tile) {
+__device__ __forceinline__ void product_ring(const Operands<SEGS>& p, const Epi& epi, uint32_t tile, uint32_t first, uint32_t end) {
   product_ring_of<F16, A_RC, B_RC, PAIR, SEGS, BM, HB, WGM, WGN, SA, SB>(
       p.a[0], p.a[SEGS - 1], p.b[0][0], p.b[0][SEGS - 1], p.b[1][0], p.b[1][SEGS - 1],
-      reinterpret_cast<const uint16_t*>(kZeroChunk), p.M, p.N, p.K, epi, tile);
+      reinterpret_cast<const uint16_t*>(kZeroChunk), p.M, p.N, p.K, epi, tile, first, end);
 }
 
 // ----------------------------------------------- few rows: the weight is read
@@ -693,7 +740,7 @@ __device__ __forceinline__ void product_ring(const Operands<SEGS>& p, const Epi&
 // apart, which the result only has to know. Eight waves of a workgroup take
 // every eighth 32-deep step of a strip of 64 columns and meet in LDS in wave
 // order; where strips are few, P workgroups share one, each a run of steps, and
-// few_join adds their partial sums in order (`part`, [P][1 or 2][M][N]).
+// join_parts adds their partial sums in order (`part`, [P][1 or 2][M][N]).
 constexpr uint32_t kFewColumns = 64, kFewWaves = 8;
 
 template <bool F16, bool PAIR, int MB, typename Epi>
@@ -845,12 +892,12 @@ __device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi
   }
 }
 
-// The P partial sums of eight columns a lane, in order, to the epilogue: 256
+// The P partial sums of eight columns a lane, in order, to the epilogue: 128
 // lanes a workgroup, along row blockIdx.x % M.
 template <bool PAIR, typename Epi>
-__device__ __forceinline__ void few_join(const float* __restrict__ part, const Epi& epi, uint32_t M, uint32_t N, uint32_t P) {
+__device__ __forceinline__ void join_parts(const float* __restrict__ part, const Epi& epi, uint32_t M, uint32_t N, uint32_t P) {
   constexpr int H = PAIR ? 2 : 1;
-  const uint32_t m = blockIdx.x % M, n = (blockIdx.x / M * 256u + threadIdx.x) * 8u;
+  const uint32_t m = blockIdx.x % M, n = (blockIdx.x / M * 128u + threadIdx.x) * 8u;
   if (n >= N) return;
   const auto f = epi.template fetch<false>(m, n);
   float v[H][8];
