@@ -371,8 +371,10 @@ struct Product {
 constexpr uint32_t kFewRows = 64;
 // Workgroups that products of few tiles are split into, by k: as many as CUs.
 constexpr uint32_t kCUs = 256;
-// Planes of at most so many results may be split (128 tiles of 128x128).
-constexpr uint64_t kSplitPlane = 1ull << 21;
+// Planes of at most so many results may be split (64 tiles of 128x128: into four and
+// more; two parts pay for the sum of their halves what they save: dx of 2048 x
+// 1024 x 4096, 128 tiles, 31 us in one launch, 25 and 5 in two parts).
+constexpr uint64_t kSplitPlane = 1ull << 20;
 
 void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   std::ostringstream ops;
@@ -565,7 +567,7 @@ void EmitBackward(const Attrs& a, bool gated, Writer* w) {
   w->Header("tca/hip/product.h");
   for (const char* d : {"M", "K", "N"}) w->Dim(d);
   // Partial rows of the bias' gradient: one for each kPartRows rows of the batch, at most kParts.
-  const uint32_t kParts = 128, kPartRows = 32;
+  const uint32_t kParts = 256, kPartRows = 16;
   if (bias) w->Dim("parts", kParts);
   if (bias) w->Dim("grads", gated ? 2 : 1);
   w->Tensor(gated ? "dh" : "dy", a.elem, "in", "M N");

@@ -109,7 +109,7 @@ __device__ __forceinline__ void norm_rows(const T* x, const W* __restrict__ gamm
         v[i][e] = v[i][e] * r * static_cast<float>(g[i][e]);
         if constexpr (BIAS) v[i][e] += static_cast<float>(b[i][e]);
       }
-      row_store<E>(y + row * C, (i * G + lane) * E, C, v[i]);
+      row_store<E, false, true>(y + row * C, (i * G + lane) * E, C, v[i]);
     }
     if constexpr (STATS) {
       if (lane == 0u) {
@@ -207,10 +207,10 @@ __device__ __forceinline__ void norm_backward_rows(const T* __restrict__ dy, con
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (i * G + lane) * E;
-      w.x[i] = row_raw<E>(x + row * C, c, C);
-      w.dy[i] = row_raw<E>(dy + row * C, c, C);
+      w.x[i] = row_raw<E, false, true>(x + row * C, c, C);
+      w.dy[i] = row_raw<E, false, true>(dy + row * C, c, C);
       // dres may be dx: this row's elements are written by the lanes that read them.
-      if constexpr (RES) w.res[i] = row_raw<E>(dres + row * C, c, C);
+      if constexpr (RES) w.res[i] = row_raw<E, false, true>(dres + row * C, c, C);
     }
   };
   Row next;

@@ -16,13 +16,13 @@ constexpr int kRowE = 16 / static_cast<int>(sizeof(T));  // values per 16-byte v
 // the end of the row is loaded from the end's last 16 bytes instead and is
 // moved into place by row_fix, which waits for it and so is called where the
 // values are used. Rows of less than 16 bytes are gathered. WHOLE: all of the
-// values lie in the row.
+// values lie in the row. NT: not kept in the caches.
 template <typename T>
 __device__ __forceinline__ uint32_t row_at(uint32_t c, uint32_t C) {
   const uint32_t last = C >= static_cast<uint32_t>(kRowE<T>) ? C - kRowE<T> : 0u;
   return c < last ? c : last;
 }
-template <int E, bool WHOLE = false, typename T>
+template <int E, bool WHOLE = false, bool NT = false, typename T>
 __device__ __forceinline__ vec<T, E> row_raw(const T* row, uint32_t c, uint32_t C) {
   constexpr int P = kRowE<T>;
   static_assert(E % P == 0, "whole pieces");
@@ -32,7 +32,7 @@ __device__ __forceinline__ vec<T, E> row_raw(const T* row, uint32_t c, uint32_t 
 #pragma unroll
   for (int k = 0; k < E / P; ++k) {
     if (WHOLE || C >= static_cast<uint32_t>(P)) {
-      r.piece[k] = load_vec_any<T, P, false>(row + (WHOLE ? c + k * P : row_at<T>(c + k * P, C)));
+      r.piece[k] = load_vec_any<T, P, NT>(row + (WHOLE ? c + k * P : row_at<T>(c + k * P, C)));
     } else {
 #pragma unroll
       for (int e = 0; e < P; ++e) r.piece[k].set(e, static_cast<uint32_t>(e) < C ? row[e] : static_cast<T>(0.0f));
@@ -87,13 +87,13 @@ __device__ __forceinline__ void row_load(const T* row, uint32_t c, uint32_t C, f
   for (int e = 0; e < E; ++e) f[e] = static_cast<float>(v[e]);
 }
 // ... and back, rounded to nearest once.
-template <int E, bool WHOLE = false, typename T>
+template <int E, bool WHOLE = false, bool NT = false, typename T>
 __device__ __forceinline__ void row_store(T* row, uint32_t c, uint32_t C, const float (&f)[E]) {
   if (WHOLE || (c < C && C - c >= static_cast<uint32_t>(E))) {
     vec<T, E> v;
 #pragma unroll
     for (int e = 0; e < E; ++e) v.set(e, static_cast<T>(f[e]));
-    store_vec_any<T, E, false>(row + c, v);
+    store_vec_any<T, E, NT>(row + c, v);
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e)
