@@ -157,7 +157,11 @@ int tca_program_selected(tca_program p, const tca_tensor* tensors, uint32_t n_te
  * calls on one stream from several threads serialize (a larger launch
  * synchronizes the stream before it replaces the buffer). The first launch
  * that needs a workspace allocates (hipMalloc), so it cannot be captured
- * into a HIP graph. */
+ * into a HIP graph: on a stream that is being captured, a launch that would
+ * have to allocate fails with TCA_ERR_INVALID before anything is queued. A
+ * workspace that a captured launch uses is kept until unload, also when a
+ * larger launch outgrows it. Graphs captured on one stream share its
+ * workspace as the launches on it do: replay them in turn. */
 int tca_program_launch(tca_program p, const tca_tensor* tensors, uint32_t n_tensors,
                        const uint32_t* free_dims, uint32_t n_free_dims,
                        const double* scalars, uint32_t n_scalars, tca_stream_t stream);

@@ -110,6 +110,7 @@ struct tca_program_s {
   struct Workspace {
     void* ptr = nullptr;
     size_t bytes = 0;
+    bool captured = false;  // a graph holds its address: kept until unload
   };
   // Everything a launch decides from the shapes alone, kept for the last
   // shape launched: a repeat launch at that shape compares the shapes,
@@ -139,7 +140,8 @@ struct tca_program_s {
   // launched on: launches on one stream are ordered and may share it,
   // launches on different streams may overlap and must not.
   std::map<tca_stream_t, Workspace> workspaces;
-  std::mutex mu;  // guards `workspaces` and `prepared`
+  std::vector<void*> retired;  // outgrown workspaces that a graph still addresses
+  std::mutex mu;  // guards `workspaces`, `retired` and `prepared`
   std::shared_ptr<const Prepared> prepared;
   std::string plan_text;  // tca_program_plan_text's buffer, filled on first request
 };
@@ -379,6 +381,10 @@ int tca_program_unload(tca_program p) {
     hipError_t e = hipFree(kv.second.ptr);
     if (e != hipSuccess && rc == TCA_OK) rc = hip_fail(e, "hipFree(workspace)");
   }
+  for (void* r : p->retired) {
+    hipError_t e = hipFree(r);
+    if (e != hipSuccess && rc == TCA_OK) rc = hip_fail(e, "hipFree(workspace)");
+  }
   if (p->mod != nullptr) {
     hipError_t e = hipModuleUnload(p->mod);
     if (e != hipSuccess && rc == TCA_OK) rc = hip_fail(e, "hipModuleUnload");
@@ -542,6 +548,18 @@ int prepare_launch(tca_program p, const tca_tensor* tensors, uint32_t n_tensors,
   return TCA_OK;
 }
 
+// Whether `stream` records its work into a graph. A query that fails (the
+// default stream while another stream is captured) leaves no error behind:
+// the launch itself reports what is wrong with it.
+bool is_capturing(tca_stream_t stream) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &st) != hipSuccess) {
+    (void)hipGetLastError();
+    return false;
+  }
+  return st != hipStreamCaptureStatusNone;
+}
+
 // Whether a launch with these arguments repeats the prepared shape with
 // usable pointers; anything else takes the slow path, which reports the
 // error a mismatch deserves.
@@ -607,8 +625,19 @@ int launch_program(tca_program p, const tca_tensor* tensors, uint32_t n_tensors,
   } else if (pr->ws_bytes > 0) {
     lk.lock();
     tca_program_s::Workspace& w = p->workspaces[stream];
+    const bool capturing = is_capturing(stream);
     if (w.bytes < pr->ws_bytes) {
-      if (w.ptr != nullptr) {
+      // An allocation would end the capture; nothing has been queued yet.
+      if (capturing)
+        return fail(TCA_ERR_INVALID,
+                    "program_launch: program %s needs %zu bytes of workspace on a stream that is being captured and has "
+                    "%zu (launch it there once at these dims before the capture)",
+                    pl.name.c_str(), pr->ws_bytes, w.bytes);
+      if (w.captured) {
+        // A captured launch addresses the smaller workspace: its replays keep it.
+        p->retired.push_back(w.ptr);
+        w = tca_program_s::Workspace{};
+      } else if (w.ptr != nullptr) {
         // Kernels queued on this stream may still use the smaller workspace.
         TCA_HIP_TRY(hipStreamSynchronize(static_cast<hipStream_t>(stream)));
         TCA_HIP_TRY(hipFree(w.ptr));
@@ -618,6 +647,7 @@ int launch_program(tca_program p, const tca_tensor* tensors, uint32_t n_tensors,
       TCA_HIP_TRY(hipMalloc(&w.ptr, pr->ws_bytes));
       w.bytes = pr->ws_bytes;
     }
+    w.captured |= capturing;
     ws = w.ptr;
   }
 

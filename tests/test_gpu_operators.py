@@ -502,6 +502,45 @@ def test_sublayer_captured_and_replayed(gpu):
             assert torch.equal(v, want[k]), k
 
 
+def test_captured_workspace_outlives_a_larger_launch(gpu):
+    """A graph keeps the workspace its launches were captured with when a
+    later launch on that stream needs a larger one; and a launch that would
+    have to allocate while its stream is captured is refused, the capture
+    going on."""
+    g = gen_of("capws")
+    p = compiler.compile_program(operators.layer_norm_backward("bf16", residual=True))  # no workspaces yet
+
+    def tensors(R, C):
+        x, dy, dres = (rand(g, (R, C), "bf16") for _ in range(3))
+        return [dy, x, rand(g, (C,), "bf16"), x.float().mean(1), x.float().std(1).reciprocal(), dres, empty((R, C), "bf16"),
+                empty((C,), "bf16"), empty((C,), "bf16")]
+
+    small, large = tensors(500, 300), tensors(700, 3000)
+    p.launch(small)
+    torch.cuda.synchronize()
+    want = [t.clone() for t in small[6:]]
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(_lib.TcaError, match="being captured"):
+            p.launch(small)
+    with torch.cuda.stream(stream):
+        p.launch(small)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        p.launch(small)
+    for _ in range(3):
+        with torch.cuda.stream(stream):
+            p.launch(large)
+        torch.cuda.synchronize()
+        for t in small[6:]:
+            t.fill_(-1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, w) for t, w in zip(small[6:], want))
+
+
 def test_two_streams_at_once(gpu):
     """One program on two streams: each has a workspace of its own."""
     a, b = Sublayer(300, 128, 344), Sublayer(270, 256, 200)
