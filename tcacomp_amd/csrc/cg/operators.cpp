@@ -406,14 +406,14 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   auto parts = [&](uint32_t least, const std::string& blocks) {
     return "tca::hip::col_split(p.K, " + blocks + ", " + std::to_string(least) + "u, " + std::to_string(kCUs) + "u)";
   };
-  auto join = [&](const std::string& suffix, const std::string& P, const std::string& record, std::vector<std::string> records,
-                  const std::string& of) {
+  auto join = [&](const std::string& suffix, uint32_t slices, const std::string& P, const std::string& record,
+                  std::vector<std::string> records, const std::string& of) {
     Writer::Kernel j;
     j.suffix = p.suffix + suffix;
     j.params = p.params + " " + part;
-    j.block = 128;
-    j.body = ops.str() + "  tca::hip::join_parts<" + pair + ">(" + part + ", epi, p.M, p.N, " + P + ");\n";
-    j.grid = p.M + "/1 " + p.N + "/1024";
+    j.block = 32u * slices;
+    j.body = ops.str() + "  tca::hip::join_parts<" + pair + ", " + std::to_string(slices) + "u>(" + part + ", epi, p.M, p.N, " + P + ");\n";
+    j.grid = p.M + "/1 " + p.N + "/256";
     j.records = std::move(records);
     j.records.push_back(record);
     j.detail = p.what + ", the partial sums of " + of + " (P > 1 only)";
@@ -445,7 +445,7 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
       w->Add(k);
       from = 16u * blocks + 1u;
     }
-    join("_fewjoin", P, split(least, terms, "1"), {When("M", 1, kFewRows)}, "few rows");
+    join("_fewjoin", 8, P, split(least, terms, "1"), {When("M", 1, kFewRows)}, "few rows");
   }
   // Rows of whole 16-byte chunks, of both operands, go straight into LDS.
   std::vector<std::string> aligned, odd;
@@ -479,7 +479,7 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
     k.records = with(records, {split(least, terms, "0"), small_plane});
     k.detail = p.what + ", " + detail + ", k over P workgroups (at most " + std::to_string(kSplitPlane) + " results)";
     w->Add(k);
-    join(suffix + "join", P, split(least, terms, "1"), with(records, {small_plane}), detail);
+    join(suffix + "join", 4, P, split(least, terms, "1"), with(records, {small_plane}), detail);
   };
   few_tiles("_k", "product_ring<" + targs + ", 128, 64, 2, 2, 5, 5>", 256, 128, aligned, "tiles of 128x128, direct to LDS");
   Writer::Kernel k;
@@ -600,6 +600,7 @@ void EmitBackward(const Attrs& a, bool gated, Writer* w) {
     Writer::Kernel k;
     k.suffix = "_slope";
     k.params = tensors + "bias_part M N";
+    k.block = 1024;
     k.body = f + "  tca::hip::slope_columns(f, bias_part, M, N, " + parts + ");\n";
     k.grid = "N/512 M/" + std::to_string(kPartRows) + ":" + std::to_string(kParts);
     k.detail = "gradients of the pre-activations, partial sums of the bias' gradient";

@@ -765,7 +765,7 @@ __device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi
     u32x4 x[MB];
   };
   Step st[D];
-  auto load = [&](Step& s, uint32_t t) {  // a step past the end re-reads the last rows; it is not used
+  auto load = [&](Step& s, uint32_t t) {
     const uint32_t k0 = t * 32u + 8u * g;
 #pragma unroll
     for (int h = 0; h < H; ++h)
@@ -827,7 +827,8 @@ __device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi
   const uint32_t t0 = first + wave;
   if (t0 < end) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) load(st[d], t0 + d * kFewWaves);
+    for (int d = 0; d < D; ++d)
+      if (t0 + d * kFewWaves < end) load(st[d], t0 + d * kFewWaves);
     for (uint32_t t = t0; t < end; t += D * kFewWaves) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
@@ -892,33 +893,53 @@ __device__ __forceinline__ void product_few(const Operands<1>& p, const Epi& epi
   }
 }
 
-// The P partial sums of eight columns a lane, in order, to the epilogue: 128
-// lanes a workgroup, along row blockIdx.x % M.
-template <bool PAIR, typename Epi>
+// The P partial sums of eight columns a lane, in order, to the epilogue: 32
+// chunks of row blockIdx.x % M by SLICES slices of the partials a workgroup,
+// four partials of a lane in flight (past the end, the last one again). With a
+// lane adding all of them, 25 partials of one row took 22 us (8 slices: 6);
+// planes of tiles have fewer partials and many rows (940 x 1040 by 4: 8.2 us with
+// 8 slices, 5 with 4).
+template <bool PAIR, uint32_t SLICES, typename Epi>
 __device__ __forceinline__ void join_parts(const float* __restrict__ part, const Epi& epi, uint32_t M, uint32_t N, uint32_t P) {
   constexpr int H = PAIR ? 2 : 1;
-  const uint32_t m = blockIdx.x % M, n = (blockIdx.x / M * 128u + threadIdx.x) * 8u;
-  if (n >= N) return;
-  const auto f = epi.template fetch<false>(m, n);
+  __shared__ __attribute__((aligned(16))) float join[SLICES][H][32][8];
+  const uint32_t i = threadIdx.x & 31u, slot = threadIdx.x >> 5;
+  const uint32_t m = blockIdx.x % M, n = (blockIdx.x / M * 32u + i) * 8u;
   float v[H][8];
 #pragma unroll
   for (int h = 0; h < H; ++h)
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[h][e] = 0.0f;
-  for (uint32_t p = 0; p < P; p += 4u) {  // four at a time in flight; past the end, the last one again
-    float s[4][H][8];
+  if (n < N)
+    for (uint32_t p = slot; p < P; p += 4u * SLICES) {
+      vec<float, 8> s[4][H];
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i)
+      for (uint32_t k = 0; k < 4u; ++k)
 #pragma unroll
-      for (int h = 0; h < H; ++h)
-        row_load<8>(part + (static_cast<uint64_t>((p + i < P ? p + i : P - 1u) * H + h) * M + m) * N, n, N, s[i][h]);
+        for (int h = 0; h < H; ++h)
+          s[k][h] = row_raw<8>(part + (static_cast<uint64_t>((p + SLICES * k < P ? p + SLICES * k : P - 1u) * H + h) * M + m) * N, n, N);
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i)
+      for (uint32_t k = 0; k < 4u; ++k)
 #pragma unroll
-      for (int h = 0; h < H; ++h)
+        for (int h = 0; h < H; ++h) {
+          row_fix<8>(s[k][h], n, N);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[h][e] = p + i < P ? v[h][e] + s[i][h][e] : v[h][e];
-  }
+          for (int e = 0; e < 8; ++e) v[h][e] = p + SLICES * k < P ? v[h][e] + s[k][h][e] : v[h][e];
+        }
+    }
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) join[slot][h][i][e] = v[h][e];
+  __syncthreads();
+  if (slot != 0u || n >= N) return;
+  const auto f = epi.template fetch<false>(m, n);
+#pragma unroll
+  for (uint32_t s = 1; s < SLICES; ++s)
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[h][e] += join[s][h][i][e];
   if constexpr (PAIR) epi.template store<false>(m, n, f, v[0], v[1]);
   else epi.template store<false>(m, n, f, v[0]);
 }
@@ -978,29 +999,30 @@ __device__ __forceinline__ void slope_flat(const Slope<T, ACT, GATED>& f, uint32
 }
 
 // ... with the column sums of a bias' gradient, of the values before they are
-// rounded: 512 columns by 4 rows a workgroup, over row chunk p of P, four rows
-// of a lane in flight; `part` is [P][1 + GATED][N].
+// rounded: 512 columns by 16 rows a workgroup of 1024 lanes, over row chunk p of
+// P, two rows of a lane in flight; `part` is [P][1 + GATED][N]. (Four rows a lane one
+// after the other take a wave 9 us, however few there are.)
 template <typename T, int ACT, bool GATED>
 __device__ __forceinline__ void slope_columns(const Slope<T, ACT, GATED>& f, float* __restrict__ part, uint32_t M,
                                               uint32_t N, uint32_t P) {
-  constexpr uint32_t AHEAD = 4;
-  __shared__ float join[4][512];
+  constexpr uint32_t AHEAD = 2, SLOTS = 16;
+  __shared__ float join[SLOTS][512];
   const uint32_t p = blockIdx.x % P, c0 = blockIdx.x / P * 512u, c = c0 + lane_id() * 8u, slot = wave_id();
   const uint64_t rows = (M - 1u) / P + 1u, first = p * rows, last = first + rows < M ? first + rows : M;
   float s0[8], s1[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) s0[e] = s1[e] = 0.0f;
   if (c < N)
-    for (uint64_t r = first + slot; r < last; r += 4u * AHEAD) {
+    for (uint64_t r = first + slot; r < last; r += SLOTS * AHEAD) {
       typename Slope<T, ACT, GATED>::Raw raw[AHEAD];
 #pragma unroll
       for (uint32_t k = 0; k < AHEAD; ++k)
-        if (r + 4u * k < last) raw[k] = f.load((r + 4u * k) * N, c, N);
+        if (r + SLOTS * k < last) raw[k] = f.load((r + SLOTS * k) * N, c, N);
 #pragma unroll
       for (uint32_t k = 0; k < AHEAD; ++k) {
-        if (r + 4u * k >= last) break;
+        if (r + SLOTS * k >= last) break;
         float f0[8], f1[8];
-        f.store(raw[k], (r + 4u * k) * N, c, N, f0, f1);
+        f.store(raw[k], (r + SLOTS * k) * N, c, N, f0, f1);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           s0[e] += f0[e];
@@ -1015,8 +1037,12 @@ __device__ __forceinline__ void slope_columns(const Slope<T, ACT, GATED>& f, flo
 #pragma unroll
     for (int e = 0; e < 8; ++e) join[slot][lane_id() * 8u + e] = q == 0u ? s0[e] : s1[e];
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 512u && c0 + i < N; i += 256u)
-      part[(static_cast<uint64_t>(p) * Q + q) * N + c0 + i] = ((join[0][i] + join[1][i]) + join[2][i]) + join[3][i];
+    if (threadIdx.x < 512u && c0 + threadIdx.x < N) {
+      float v = join[0][threadIdx.x];
+#pragma unroll
+      for (uint32_t s = 1; s < SLOTS; ++s) v += join[s][threadIdx.x];
+      part[(static_cast<uint64_t>(p) * Q + q) * N + c0 + threadIdx.x] = v;
+    }
   }
 }
 
