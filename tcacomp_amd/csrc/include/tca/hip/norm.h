@@ -50,29 +50,48 @@ __device__ __forceinline__ void norm_group_sums(float (&v)[S], float* lds) {
   }
 }
 
+// What vector i of a wave's lanes, of groups of G, holds of rows of C: nothing,
+// part of its places, or all. The same for every lane of the wave.
+enum { kNormNone, kNormPart, kNormAll };
+template <int G, int E>
+__device__ __forceinline__ int norm_holds(int i, uint32_t C) {
+  const uint32_t wave = G > 64 ? static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) % (G / 64) : 0u;
+  const uint32_t first = (i * G + wave * 64u) * E, span = (G < 64 ? G : 64) * E;
+  return first >= C ? kNormNone : C - first < span ? kNormPart : kNormAll;
+}
+
 // Rows by groups of G lanes, at most NV vectors per lane (C <= G NV E), the
 // workgroups walking them with the grid as their stride: a row's loads are
-// issued a row ahead, and gamma and beta are read once.
+// issued a row ahead, and gamma and beta are read once (in rows of 32 16-bit
+// values a lane again for every row, out of the L2: registers for both spill).
 template <typename T, typename W, int G, int NV, bool BIAS, bool STATS>
 __device__ __forceinline__ void norm_rows(const T* x, const W* __restrict__ gamma, const W* __restrict__ beta, T* y,
                                           float* __restrict__ mean, float* __restrict__ rstd, uint32_t R, uint32_t C,
                                           float eps) {
   constexpr int E = kRowE<T>, BLOCK = G < 256 ? 256 : G, GROUPS = BLOCK / G;
+  constexpr bool HELD = BLOCK < 1024 || NV * E < 32;
   __shared__ float lds[2][2][BLOCK / 64];
   const uint32_t lane = threadIdx.x % G;
   uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * GROUPS;  // the workgroup's first row
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * GROUPS, grp = threadIdx.x / G;
   vec<T, E> next[NV];
   vec<W, E> g[NV], b[NV];
+  int holds[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) holds[i] = norm_holds<G, E>(i, C);
   auto load = [&](uint64_t row) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) next[i] = row_raw<E>(x + row * C, (i * G + lane) * E, C);
+    for (int i = 0; i < NV; ++i)
+      if (holds[i] != kNormNone) next[i] = row_raw<E>(x + row * C, (i * G + lane) * E, C);
   };
-  if (r0 + grp < R) load(r0 + grp);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  auto weights = [&](int i) {
     g[i] = row_vec<E>(gamma, (i * G + lane) * E, C);
     if constexpr (BIAS) b[i] = row_vec<E>(beta, (i * G + lane) * E, C);
+  };
+  if (r0 + grp < R) load(r0 + grp);
+  if constexpr (HELD) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) weights(i);
   }
   // r0 is the same for every group: all of them reach the barriers.
   for (uint32_t turn = 0u; r0 < R; r0 += step, ++turn) {
@@ -81,35 +100,46 @@ __device__ __forceinline__ void norm_rows(const T* x, const W* __restrict__ gamm
     float s[1] = {0.0f}, q[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      row_fix<E>(next[i], (i * G + lane) * E, C);
+      if (holds[i] == kNormPart) row_fix<E>(next[i], (i * G + lane) * E, C);
 #pragma unroll
       for (int e = 0; e < E; ++e) v[i][e] = static_cast<float>(next[i][e]);
     }
     if (row + step < R) load(row + step);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
+      if (holds[i] != kNormNone) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) s[0] += v[i][e];
+        for (int e = 0; e < E; ++e) s[0] += v[i][e];
+      }
     norm_group_sums<G>(s, lds[turn & 1u][0]);
     const float m = s[0] / static_cast<float>(C);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      if (holds[i] == kNormNone) continue;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        v[i][e] -= m;
-        if ((i * G + lane) * E + e < C) q[0] = __builtin_fmaf(v[i][e], v[i][e], q[0]);
+      for (int e = 0; e < E; ++e) v[i][e] -= m;
+      if (holds[i] == kNormPart) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if ((i * G + lane) * E + e >= C) v[i][e] = 0.0f;
       }
+#pragma unroll
+      for (int e = 0; e < E; ++e) q[0] = __builtin_fmaf(v[i][e], v[i][e], q[0]);
+    }
     norm_group_sums<G>(q, lds[turn & 1u][1]);
     const float r = 1.0f / __builtin_sqrtf(q[0] / static_cast<float>(C) + eps);
     if (row >= R) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if (holds[i] == kNormNone) continue;
+      if constexpr (!HELD) weights(i);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         v[i][e] = v[i][e] * r * static_cast<float>(g[i][e]);
         if constexpr (BIAS) v[i][e] += static_cast<float>(b[i][e]);
       }
-      row_store<E, false, true>(y + row * C, (i * G + lane) * E, C, v[i]);
+      if (holds[i] == kNormAll) row_store<E, true, true>(y + row * C, (i * G + lane) * E, C, v[i]);
+      else row_store<E, false, true>(y + row * C, (i * G + lane) * E, C, v[i]);
     }
     if constexpr (STATS) {
       if (lane == 0u) {
@@ -201,12 +231,16 @@ __device__ __forceinline__ void norm_backward_rows(const T* __restrict__ dy, con
   };
   uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * GROUPS;
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * GROUPS;
+  int holds[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) holds[i] = norm_holds<G, E>(i, C);
   auto load = [&](Row& w, uint64_t row) {
     w.m = mean[row];
     w.rs = rstd[row];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (i * G + lane) * E;
+      if (holds[i] == kNormNone) continue;
       w.x[i] = row_raw<E, false, true>(x + row * C, c, C);
       w.dy[i] = row_raw<E, false, true>(dy + row * C, c, C);
       // dres may be dx: this row's elements are written by the lanes that read them.
@@ -231,6 +265,7 @@ __device__ __forceinline__ void norm_backward_rows(const T* __restrict__ dy, con
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (i * G + lane) * E;
+      if (holds[i] != kNormPart) continue;
       row_fix<E>(now.x[i], c, C);
       row_fix<E>(now.dy[i], c, C);
       if constexpr (RES) row_fix<E>(now.res[i], c, C);
@@ -239,21 +274,24 @@ __device__ __forceinline__ void norm_backward_rows(const T* __restrict__ dy, con
     float s[2] = {0.0f, 0.0f};
     if (live) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i) {
+        if (holds[i] == kNormNone) continue;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
+        for (int e = 0; e < E; ++e) {  // (past the end of the row dy is 0, and so are t and t h)
           const float h = (static_cast<float>(now.x[i][e]) - now.m) * now.rs, d = static_cast<float>(now.dy[i][e]);
           dg[i][e] = __builtin_fmaf(d, h, dg[i][e]);
           db[i][e] += d;
           const float t = d * static_cast<float>(g[i][e]);
           s[0] += t;
-          if ((i * G + lane) * E + e < C) s[1] = __builtin_fmaf(t, h, s[1]);
+          s[1] = __builtin_fmaf(t, h, s[1]);
         }
+      }
     }
     norm_group_sums<G>(s, sums[turn & 1u]);
     if (!live) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if (holds[i] == kNormNone) continue;
       float o[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -262,7 +300,8 @@ __device__ __forceinline__ void norm_backward_rows(const T* __restrict__ dy, con
         o[e] = (t - (s[0] + h * s[1]) * inv) * now.rs;
         if constexpr (RES) o[e] += static_cast<float>(now.res[i][e]);
       }
-      row_store<E>(dx + row * C, (i * G + lane) * E, C, o);
+      if (holds[i] == kNormAll) row_store<E, true>(dx + row * C, (i * G + lane) * E, C, o);
+      else row_store<E>(dx + row * C, (i * G + lane) * E, C, o);
     }
   }
   // The groups' sums, in group order.
