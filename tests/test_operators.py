@@ -154,6 +154,89 @@ def test_partial_rows_are_as_many_as_the_join_adds():
             assert grid == min(-(-R // (512 // lanes)), 256)
 
 
+def product_kernels(M, N, K, few, odd, half=1):
+    """{suffix: workgroups} of one product of M x K by K x N (half 2: of two),
+    by the rules restated, each as it is launched."""
+    up = lambda a, b: -(-a // b)  # noqa: E731
+
+    def shared(suffix, blocks, least):
+        P = max(1, min(up(K, least), 256 // blocks))
+        return {suffix: blocks * P, **({suffix.rstrip("0123456789") + "join": M * up(N, 256)} if P > 1 else {})}
+
+    def tiles(rows, cols):
+        return up(M, rows) * up(N, cols // half)
+
+    if few and M <= 64:
+        return shared("_few%d" % (16 if M <= 16 else 32 if M <= 32 else 64), up(N, 64), 256)
+    if M * N <= 1 << 20:
+        return shared("_o", tiles(64, 128), 512) if odd else shared("_k", tiles(128, 128), 512)
+    if odd:
+        return {"_a": tiles(128, 128)} if tiles(128, 128) >= 256 else {"": tiles(64, 128)}
+    for form, rows, cols, least, of in (("_l", 256, 256, 385, (256, 256)), ("_m", 256, 128, 257, (256, 256)),
+                                        ("_l", 256, 256, 192, (256, 256)), ("_m", 256, 128, 192, (256, 128)),
+                                        ("_s", 128, 128, 257, (128, 128))):
+        if tiles(*of) >= least:
+            return {form: tiles(rows, cols)}
+    return {"_r": tiles(128, 128)}
+
+
+def launched(p, plan, tensors, dims):
+    """{suffix: workgroups} of a launch: the selected kernels, or the first of
+    their forms whose bounds hold (plan: its kernel and form lines)."""
+    out = {}
+    for symbol, grid in selected(p, tensors).items():
+        for name, bounds in plan[symbol]:
+            counts = [(least, [dims[t.split("/")[0]] for t in terms], [int(t.split("/")[1]) for t in terms]) for least, terms in bounds]
+            sizes = [-(-d[0] // q[0]) * -(-d[1] // q[1]) for _, d, q in counts]
+            if all(size >= least for size, (least, _, _) in zip(sizes, counts)):
+                symbol, grid = name, sizes[0]
+                break
+        out[symbol[len("tca_" + p.name):]] = grid
+    return out
+
+
+def forms(op):
+    """{kernel: [(form, [(least, terms)])]} and all names of an operator's plan."""
+    plan, last = {}, None
+    for line in op.emit().plan.splitlines():
+        w = line.split()
+        if w and w[0] == "kernel":
+            last = w[1]
+            plan[last] = []
+        elif w and w[0] == "form":
+            assert w[2:4] == ["0", "2"] and w[5] == w[9] == "2" and len(w) == 12, line
+            plan[last].append((w[1], [(int(w[4]), w[6:8]), (int(w[8]), w[10:12])]))
+    return plan
+
+
+SIZES = [1, 7, 8, 16, 17, 64, 65, 72, 128, 255, 512, 1000, 1024, 1032, 2048, 3600, 4096, 7297, 8192, 20000]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_every_product_takes_one_kernel(gated):
+    """Forward and backward: one kernel for each product, with its join where
+    k is split and only there, and as many workgroups as the kernel counts."""
+    fop = (operators.gated if gated else operators.linear)("bf16", act="silu")
+    bop = (operators.gated_backward if gated else operators.linear_backward)("bf16", act="silu")
+    fwd, bwd, fplan, bplan = compiled(fop), compiled(bop), forms(fop), forms(bop)
+    n = 2 if gated else 1
+    seen = set()
+    for M, K, N in itertools.product(SIZES, SIZES, SIZES):
+        x, w, y, dims = desc("bf16", M, K), desc("bf16", K, N), desc("bf16", M, N), dict(M=M, K=K, N=N)
+        got = launched(fwd, fplan, [x] + [w] * n + [y], dims)
+        assert got == product_kernels(M, N, K, True, K % 8 or N % 8, half=n), dims
+        seen |= {fwd.name + s for s in got}
+        got = launched(bwd, bplan, [y, x] + [w] * n + [y] * n + [y] * n + [x] + [w] * n, dims)
+        want = {"_slope": -(-M * N // 2048)}
+        want.update({"_dx" + s: g for s, g in product_kernels(M, K, N, False, N % 8).items()})
+        want.update({"_dw" + s: g for s, g in product_kernels(K, N, M, False, K % 8 or N % 8, half=n).items()})
+        assert got == want, dims
+        seen |= {bwd.name + s for s in got}
+    # nothing in the programs that no size takes
+    for plan in (fplan, bplan):
+        assert {s[4:] for s in plan} | {f[0][4:] for of in plan.values() for f in of} <= seen
+
+
 def test_shape_contract():
     p = compiled(operators.gated("bf16", save=True))
     good = [desc("bf16", 4, 8), desc("bf16", 8, 16), desc("bf16", 8, 16)] + [desc("bf16", 4, 16)] * 3
