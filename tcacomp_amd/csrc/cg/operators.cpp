@@ -489,6 +489,15 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   k.body = body("product_ring<" + targs + ", 128, 64, 2, 2, 5, 5>");
   k.grid = tiles(128, 128);
   k.detail = p.what + ", tiles of 128x128 (256x256, 256x128 where they fill the card), 4 waves, direct to LDS";
+  // Larger tiles load less for a product, and need more of the plane to fill
+  // 256 CUs; one workgroup of 256x256 or 256x128 holds a CU, two of 128x128 with
+  // shorter rings do. Bounds by whole rounds of the card, at k = 4096 (us, bf16, _l /
+  // _m / _s / _r; products of k-contiguous and row-contiguous operands and pairs
+  // alike within 5%):
+  //   tiles of 256x256    64: 79.5 / 50.4 / 39.9 / 36.0   130: 87.3 / 102.6 / 89.5 / 97.0
+  //                       96: 82.5 / 53.2 / 53.5 / 64.5   256: 104 / 118 / 121 / 145
+  //                      272: 172 / 155 / 167 / 188       384: 191 / 179 / 202 / 244
+  //                      400: 187 / 217 / 236 / 274       512: 203 / 242 / 263 / 310
   auto form = [&](Writer::Kernel* of, const char* suffix, const std::string& what, const std::string& call, uint32_t rows,
                   uint32_t cols, uint32_t least, const std::string& terms) {
     // its grid, then the bound: at least so many tiles, of `terms`
@@ -501,20 +510,30 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   const std::string cfg_l = ring + ", 256, 128, 2, 2, 3, 2>", cfg_m = ring + ", 256, 64, 2, 2, 3, 3>", cfg_s = ring + ", 128, 64, 2, 2, 3, 2>";
   form(&k, "_l", what_l, cfg_l, 256, 256, 385, large);
   form(&k, "_m", what_m, cfg_m, 256, 128, 257, large);
-  form(&k, "_l", what_l, cfg_l, 256, 256, 192, large);
+  form(&k, "_l", what_l, cfg_l, 256, 256, 257, tall);
   form(&k, "_m", what_m, cfg_m, 256, 128, 192, tall);
   form(&k, "_s", what_s, cfg_s, 128, 128, 257, small);
   w->Add(k);
+  // (1101 x 1001 x 2049, 72 tiles of 128x128: 34 us, of 64x128 27; 132 of them 35 and
+  // 36; 432, 53 and 70.)
   few_tiles("_o", "product_any<" + targs + ", 64>", 512, 64, odd, "tiles of 64x128, any shape and alignment");
+  const std::string what_a = "tiles of 128x128, any shape and alignment", cfg_a = "product_any<" + targs + ", 128>";
   Writer::Kernel any;
-  any.suffix = p.suffix;
   any.params = p.params;
   any.block = 512;
   any.records = with(odd, {large_plane});
-  any.body = body("product_any<" + targs + ", 64>");
-  any.grid = tiles(64, 128);
-  any.detail = p.what + ", tiles of 64x128 (128x128 where they fill the card), any shape and alignment";
-  form(&any, "_a", "tiles of 128x128, any shape and alignment", "product_any<" + targs + ", 128>", 128, 128, kCUs, small);
+  if (p.pair) {  // 128 tiles and more
+    any.suffix = p.suffix + "_a";
+    any.body = body(cfg_a);
+    any.grid = small;
+    any.detail = p.what + ", " + what_a;
+  } else {
+    any.suffix = p.suffix;
+    any.body = body("product_any<" + targs + ", 64>");
+    any.grid = tiles(64, 128);
+    any.detail = p.what + ", tiles of 64x128 (128x128 from 128 tiles on), any shape and alignment";
+    form(&any, "_a", what_a, cfg_a, 128, 128, 128, small);
+  }
   w->Add(any);
 }
 

@@ -55,7 +55,7 @@ __device__ __forceinline__ void norm_group_sums(float (&v)[S], float* lds) {
 enum { kNormNone, kNormPart, kNormAll };
 template <int G, int E>
 __device__ __forceinline__ int norm_holds(int i, uint32_t C) {
-  const uint32_t wave = G > 64 ? static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) % (G / 64) : 0u;
+  const uint32_t wave = G > 64 ? static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) % (G > 64 ? G / 64 : 1) : 0u;
   const uint32_t first = (i * G + wave * 64u) * E, span = (G < 64 ? G : 64) * E;
   return first >= C ? kNormNone : C - first < span ? kNormPart : kNormAll;
 }

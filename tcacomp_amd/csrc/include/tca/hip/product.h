@@ -73,9 +73,11 @@ __device__ __forceinline__ float act_slope(float z) {
     const float d = 0.39894228040143268f * (x * e);  // |z| phi(z)
     return z < 0.0f ? q - d : z == z ? (1.0f - q) + d : z;
   } else if constexpr (ACT == kActGeluTanh) {
-    const float s = act_sigmoid(1.59576912160573071f * z * __builtin_fmaf(0.044715f * z, z, 1.0f));
-    const float du = 1.59576912160573071f * __builtin_fmaf(3.0f * 0.044715f * z, z, 1.0f);
-    return s * __builtin_fmaf(z * du, 1.0f - s, 1.0f);
+    // Held where s is 0 or 1 exactly: z^3 would pass the range, and 0 times that.
+    const float x = __builtin_fminf(__builtin_fmaxf(z, -32.0f), 32.0f);
+    const float s = act_sigmoid(1.59576912160573071f * x * __builtin_fmaf(0.044715f * x, x, 1.0f));
+    const float du = 1.59576912160573071f * __builtin_fmaf(3.0f * 0.044715f * x, x, 1.0f);
+    return z == z ? s * __builtin_fmaf(x * du, 1.0f - s, 1.0f) : z;
   } else {
     return 1.0f;
   }

@@ -387,6 +387,22 @@ def test_products_not_finite(gpu):
         assert bool((~y[bad].isfinite()).all()) and torch.equal(y[~bad], clean[~bad]), (M, K, N)
 
 
+@pytest.mark.parametrize("elem,act,bias", [("bf16", "silu", False), ("bf16", "gelu_tanh", True), ("f16", "gelu", True)])
+def test_slopes_far_out(gpu, elem, act, bias):
+    """Pre-activations of up to the type's largest value: a slope of exactly 1 or 0,
+    a value of exactly g or 0, never a product of 0 and an overflow."""
+    top = float(torch.finfo(ref.DTYPES[elem]).max)
+    far = [v for v in (200.0, 1e4, 6e4, 1e13, 1e15, 1e19, 1e25, top) if v <= top]
+    g = torch.tensor([[s * v for v in far for s in (1, -1)]], device="cuda").to(ref.DTYPES[elem])
+    N = g.shape[1]
+    one, w, x = torch.ones_like(g), rand(gen_of("far"), (8, N), elem), rand(gen_of("far"), (1, 8), elem)
+    dg, du, dx, dwg, dwu = empty((1, N), elem), empty((1, N), elem), empty((1, 8), elem), empty((8, N), elem), empty((8, N), elem)
+    db = [empty((N,), elem), empty((N,), elem)] * bias
+    program(operators.gated_backward, elem, act=act, bias=bias).launch([one, x, w, w, g, one, dg, du, dx, dwg, dwu] + db)
+    zero = torch.zeros_like(g)
+    assert torch.equal(dg, torch.where(g > 0, one, zero)) and torch.equal(du, torch.where(g > 0, g, zero)), (dg, du)
+
+
 def test_linear_in_place_residual(gpu):
     for M, K, N in ((3, 130, 200), (140, 96, 264), (260, 77, 301)):
         g = gen_of("lip", M, K, N)

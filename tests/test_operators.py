@@ -171,9 +171,9 @@ def product_kernels(M, N, K, few, odd, half=1):
     if M * N <= 1 << 20:
         return shared("_o", tiles(64, 128), 512) if odd else shared("_k", tiles(128, 128), 512)
     if odd:
-        return {"_a": tiles(128, 128)} if tiles(128, 128) >= 256 else {"": tiles(64, 128)}
+        return {"_a": tiles(128, 128)} if tiles(128, 128) >= 128 else {"": tiles(64, 128)}
     for form, rows, cols, least, of in (("_l", 256, 256, 385, (256, 256)), ("_m", 256, 128, 257, (256, 256)),
-                                        ("_l", 256, 256, 192, (256, 256)), ("_m", 256, 128, 192, (256, 128)),
+                                        ("_l", 256, 256, 257, (256, 128)), ("_m", 256, 128, 192, (256, 128)),
                                         ("_s", 128, 128, 257, (128, 128))):
         if tiles(*of) >= least:
             return {form: tiles(rows, cols)}
