@@ -11,6 +11,10 @@
  * the reference it emits code and a build recipe and does not drive the
  * device compiler itself.
  *
+ *   tcacomp operator [-o DIR] <name> [<attribute> ...]
+ * writes the same files for one operator program (include/tca_op.h; no
+ * counterpart in the reference), and without a name lists the operators.
+ *
  * Files per kernel: <kernel>.hip (the generated code object source),
  * <kernel>.plan (the launch plan tca_program_load reads beside the code
  * object). One Makefile per run (the counterpart of the reference's
@@ -33,12 +37,14 @@
 #include <sys/stat.h>
 
 #include "tca_cg.h"
+#include "tca_op.h"
 #include "tca_syntax.h"
 
 static void usage(void) {
   fprintf(stderr,
           "usage:\n"
           "  tcacomp compile [flags] <input.tca>   compile a TCA source file to HIP code objects\n"
+          "  tcacomp operator [flags] [<name> [<attribute> ...]]   emit an operator program, or list the operators\n"
           "\n"
           "flags:\n"
           "  -o string\n"
@@ -176,87 +182,86 @@ static int write_makefile(const char* dir, const char* include_dir, const built_
   return 0;
 }
 
-/* Compiles kernel i of m into dir; fills *k with what the Makefile needs. */
+/* Writes the files of emitted program `name` into dir; fills *k with what the
+ * Makefile needs. */
+static int write_kernel(tca_emit_result r, const char* name, const char* dir, built_kernel* k) {
+  char file[1024];
+  snprintf(file, sizeof file, "%s.hip", name);
+  if (write_file(dir, file, tca_emit_source(r)) != 0) return 1;
+  snprintf(file, sizeof file, "%s.plan", name);
+  if (write_file(dir, file, tca_emit_plan(r)) != 0) return 1;
+  k->name = strdup(name);
+  k->n_args = tca_emit_hipcc_argc(r);
+  k->args = calloc(k->n_args ? k->n_args : 1, sizeof(char*));
+  if (k->name == NULL || k->args == NULL) return 1;
+  for (unsigned j = 0; j < k->n_args; ++j)
+    if ((k->args[j] = strdup(tca_emit_hipcc_arg(r, j))) == NULL) return 1;
+  printf("tcacomp: compiled %s -> %s\n", name, dir);
+  return 0;
+}
+
+static void free_kernel(built_kernel* k) {
+  for (unsigned j = 0; k->args && j < k->n_args; ++j) free(k->args[j]);
+  free(k->args);
+  free(k->name);
+}
+
+/* Compiles kernel i of m into dir. */
 static int compile_kernel(tca_syntax_module m, uint32_t i, const char* target, const char* dir, built_kernel* k) {
   const char* name = tca_syntax_module_kernel_name(m, i);
   tca_builder b = NULL;
   tca_emit_result r = NULL;
-  char file[1024];
   int rc = 1;
   if (tca_syntax_module_build_kernel(m, i, &b) != TCA_OK) {
     fprintf(stderr, "tcacomp: kernel %s: %s\n", name, tca_syntax_last_error());
     return 1;
   }
-  if (tca_emit(b, NULL, target, 0, &r) != TCA_OK) {
-    fprintf(stderr, "tcacomp: kernel %s: %s\n", name, tca_builder_error(b));
-    goto out;
-  }
-  snprintf(file, sizeof file, "%s.hip", name);
-  if (write_file(dir, file, tca_emit_source(r)) != 0) goto out;
-  snprintf(file, sizeof file, "%s.plan", name);
-  if (write_file(dir, file, tca_emit_plan(r)) != 0) goto out;
-  k->name = strdup(name);
-  k->n_args = tca_emit_hipcc_argc(r);
-  k->args = calloc(k->n_args ? k->n_args : 1, sizeof(char*));
-  if (k->name == NULL || k->args == NULL) goto out;
-  for (unsigned j = 0; j < k->n_args; ++j)
-    if ((k->args[j] = strdup(tca_emit_hipcc_arg(r, j))) == NULL) goto out;
-  printf("tcacomp: compiled %s -> %s\n", name, dir);
-  rc = 0;
-out:
+  if (tca_emit(b, NULL, target, 0, &r) != TCA_OK) fprintf(stderr, "tcacomp: kernel %s: %s\n", name, tca_builder_error(b));
+  else rc = write_kernel(r, name, dir, k);
   if (r) tca_emit_free(r);
   if (b) tca_builder_free(b);
   return rc;
 }
 
+/* The flags of a command, then its arguments: flags end at the first argument
+ * that is not one. Returns the index of the first argument, -1 after a usage
+ * error. */
+static int parse_flags(int argc, char** argv, const char** out_dir, const char** target) {
+  for (int i = 0; i < argc; ++i) {
+    const char* a = argv[i];
+    if (strcmp(a, "--") == 0) return i + 1;
+    if (a[0] != '-' || strcmp(a, "-") == 0) return i;
+    const char* flag = a;
+    if (a[1] == '-' && a[2] != '\0') flag = a + 1; /* --x reads as -x */
+    const char** slot = NULL;
+    if (strcmp(flag, "-o") == 0 || strncmp(flag, "-o=", 3) == 0) slot = out_dir;
+    else if (strcmp(flag, "-target") == 0 || strncmp(flag, "-target=", 8) == 0) slot = target;
+    if (slot == NULL) {
+      fprintf(stderr, "flag provided but not defined: %s\n", a);
+      usage();
+      return -1;
+    }
+    const char* eq = strchr(flag, '=');
+    if (eq == NULL && i + 1 >= argc) {
+      fprintf(stderr, "flag needs an argument: %s\n", a);
+      usage();
+      return -1;
+    }
+    *slot = eq ? eq + 1 : argv[++i];
+  }
+  return argc;
+}
+
 static int compile(int argc, char** argv) {
   const char* out_dir = "tcacomp-out";
   const char* target = "gfx950";
-  const char* input = NULL;
-  int n_inputs = 0;
-  for (int i = 0; i < argc; ++i) {
-    const char* a = argv[i];
-    if (n_inputs > 0 || strcmp(a, "-") == 0) { /* flags end at the first argument that is not one */
-      input = a;
-      ++n_inputs;
-      continue;
-    }
-    if (strcmp(a, "--") == 0) {
-      for (++i; i < argc; ++i) {
-        input = argv[i];
-        ++n_inputs;
-      }
-      break;
-    }
-    const char* flag = a;
-    if (a[0] == '-' && a[1] == '-' && a[2] != '\0') flag = a + 1; /* --x reads as -x */
-    const char** slot = NULL;
-    const char* val = NULL;
-    if (strcmp(flag, "-o") == 0 || strncmp(flag, "-o=", 3) == 0) slot = &out_dir;
-    else if (strcmp(flag, "-target") == 0 || strncmp(flag, "-target=", 8) == 0) slot = &target;
-    if (slot != NULL) {
-      const char* eq = strchr(flag, '=');
-      if (eq) val = eq + 1;
-      else if (i + 1 < argc) val = argv[++i];
-      else {
-        fprintf(stderr, "flag needs an argument: %s\n", a);
-        usage();
-        return 2;
-      }
-      *slot = val;
-    } else if (a[0] == '-') {
-      fprintf(stderr, "flag provided but not defined: %s\n", a);
-      usage();
-      return 2;
-    } else {
-      input = a;
-      ++n_inputs;
-    }
-  }
-  if (n_inputs != 1) {
+  const int first = parse_flags(argc, argv, &out_dir, &target);
+  if (first < 0) return 2;
+  if (argc - first != 1) {
     fprintf(stderr, "tcacomp compile: exactly one input file required\n");
     return 2;
   }
+  const char* input = argv[first];
 
   tca_syntax_module m = NULL;
   if (tca_syntax_parse_module(input, &m) != TCA_OK) {
@@ -290,13 +295,39 @@ static int compile(int argc, char** argv) {
     if (rc == 0) ++done;
   }
   if (rc == 0) rc = write_makefile(out_dir, include_dir, ks, done) != 0;
-  for (unsigned i = 0; ks && i < n; ++i) {
-    for (unsigned j = 0; ks[i].args && j < ks[i].n_args; ++j) free(ks[i].args[j]);
-    free(ks[i].args);
-    free(ks[i].name);
-  }
+  for (unsigned i = 0; ks && i < n; ++i) free_kernel(&ks[i]);
   free(ks);
   tca_syntax_module_free(m);
+  return rc;
+}
+
+static int operator_(int argc, char** argv) {
+  const char* out_dir = "tcacomp-out";
+  const char* target = "gfx950";
+  const int first = parse_flags(argc, argv, &out_dir, &target);
+  if (first < 0) return 2;
+  if (first == argc) {
+    fputs(tca_op_list(), stdout);
+    return 0;
+  }
+  size_t len = 1;
+  for (int i = first + 1; i < argc; ++i) len += strlen(argv[i]) + 1;
+  char* attributes = calloc(len, 1);
+  if (attributes == NULL) return 1;
+  for (int i = first + 1; i < argc; ++i) strcat(strcat(attributes, argv[i]), " ");
+  tca_emit_result r = NULL;
+  built_kernel k = {NULL, NULL, 0};
+  char include_dir[4096];
+  int rc = 1;
+  if (tca_op_emit(argv[first], attributes, target, &r) != TCA_OK) fprintf(stderr, "tcacomp: %s\n", tca_op_last_error());
+  else if (mkdir_p(out_dir) != 0) fprintf(stderr, "tcacomp: create output dir: %s: %s\n", out_dir, strerror(errno));
+  else if (device_include_dir(include_dir, sizeof include_dir) != 0)
+    fprintf(stderr, "tcacomp: cannot locate the device headers beside libtcacomp.so\n");
+  else
+    rc = write_kernel(r, tca_op_program_name(r), out_dir, &k) != 0 || write_makefile(out_dir, include_dir, &k, 1) != 0;
+  free_kernel(&k);
+  free(attributes);
+  if (r) tca_emit_free(r);
   return rc;
 }
 
@@ -306,6 +337,7 @@ int main(int argc, char** argv) {
     return 2;
   }
   if (strcmp(argv[1], "compile") == 0) return compile(argc - 2, argv + 2);
+  if (strcmp(argv[1], "operator") == 0) return operator_(argc - 2, argv + 2);
   if (strcmp(argv[1], "help") == 0 || strcmp(argv[1], "-h") == 0 || strcmp(argv[1], "--help") == 0) {
     usage();
     return 0;

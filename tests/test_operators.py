@@ -3,12 +3,13 @@ against differences and autograd, the emitted programs, which kernel a size
 takes, and the refusals of the C ABI."""
 import ctypes
 import itertools
+import subprocess
 
 import pytest
 import torch
 
 import operators_ref as ref
-from tcacomp_amd import _lib, compiler, operators
+from tcacomp_amd import _lib, build, compiler, operators
 from tcacomp_amd.compiler import TensorDesc
 from tcacomp_amd.pkg import TBF16, BuildError
 
@@ -248,3 +249,22 @@ def test_shape_contract():
         assert p.check(t) == _lib.TCA_ERR_SHAPE
     assert p.check(good[:-1]) == _lib.TCA_ERR_INVALID
     assert p.check([TensorDesc(8, (4, 8), 2)] + good[1:]) == _lib.TCA_ERR_INVALID
+
+
+def test_the_driver_emits_operators(tmp_path):
+    """tcacomp operator: the files of the program, word for word, with a Makefile
+    of its own hipcc line; the list; refusals."""
+    cli = lambda *a: subprocess.run([build.CLI] + list(a), capture_output=True, text=True)  # noqa: E731
+    r = cli("operator")
+    assert r.returncode == 0 and r.stdout == _lib.lib().tca_op_list().decode()
+    op = operators.linear("bf16", act="gelu", bias=True)
+    r = cli("operator", "-o", str(tmp_path), "linear", "elem=bf16", "act=gelu", "bias")
+    assert r.returncode == 0 and r.stdout == "tcacomp: compiled %s -> %s\n" % (op.name, tmp_path), r.stderr
+    e = op.emit()
+    assert (tmp_path / (op.name + ".hip")).read_text() == e.source and (tmp_path / (op.name + ".plan")).read_text() == e.plan
+    r = subprocess.run(["make", "-n", "-C", str(tmp_path)], capture_output=True, text=True)
+    assert r.returncode == 0 and all(f in r.stdout for f in e.hipcc) and op.name + ".hip" in r.stdout
+    for args, code, word in ((("nothing", "elem=bf16"), 1, "nothing"), (("linear", "elem=f32"), 1, "elem=f32"),
+                             (("-target", "sm_86", "linear", "elem=bf16"), 1, "sm_86"), (("-x", "linear"), 2, "-x"), (("-o",), 2, "-o")):
+        r = cli("operator", *args)
+        assert r.returncode == code and word in r.stderr and not r.stdout, (args, r.stderr)
