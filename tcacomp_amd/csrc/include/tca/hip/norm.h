@@ -18,6 +18,12 @@
 // the grid as its stride, sums its rows' terms in registers, joins its groups
 // in LDS and writes one partial row; join_partials adds the partial rows, always
 // in the same order.
+//
+// Measured: forward f32 [32768, 1024] with the statistics 46 to 48 us (268 MB, 5.6 to
+// 5.8 TB/s), f16 [3000, 8000] 24, [1618, 16880] 31; backward bf16 [8192, 4096]
+// with a residual 43 to 45 us (268 MB, 6.0 TB/s) and 4 to 5 for the join. Streaming
+// stores (forward) and loads (backward) took 5 and 8% off, loads a row ahead
+// and joins of 1024 lanes 10 and 30%.
 #ifndef TCA_HIP_NORM_H_
 #define TCA_HIP_NORM_H_
 
@@ -324,7 +330,8 @@ __device__ __forceinline__ void norm_backward_rows(const T* __restrict__ dy, con
 }
 
 // dx of rows longer than norm_backward_rows takes, one per workgroup of 1024
-// lanes: the two sums in one read, the map in a second.
+// lanes: the two sums in one read, the map in a second. (f16 [1901, 24912] with a
+// residual 88 us, and 38 for the columns' pass over the same rows.)
 template <typename T, typename W, bool RES>
 __device__ __forceinline__ void norm_backward_long(const T* __restrict__ dy, const T* __restrict__ x,
                                                    const W* __restrict__ gamma, const float* __restrict__ mean,
