@@ -93,8 +93,8 @@ bool ParseAttrs(const Spec& s, const std::string& text, Attrs* a, std::string* e
       ok = Has(s.elems, value);
       a->elem = value;
     } else if (key == "weight") {
-      ok = s.weight && (value == "f32" || value == "elem");
-      if (value == "f32") a->weight = value;
+      ok = s.weight && value == "f32";
+      a->weight = value;
     } else if (key == "act") {
       ok = s.act && Has(Acts(), value);
       a->act = value;

@@ -575,6 +575,37 @@ def test_two_streams_at_once(gpu):
             assert torch.equal(v, w[k]), k
 
 
+@pytest.mark.parametrize("N", [32768, 32767])
+def test_planes_past_32_bit_offsets(gpu, N):
+    """70000 rows: 2.3e9 elements, 4.6e9 bytes; the rows round the 2^31st element
+    and the last ones, and the columns' sums over all rows."""
+    M, K = 70000, 64
+    g = gen_of("far", N)
+    big = lambda: torch.empty((M, N), device="cuda", dtype=torch.bfloat16).normal_(generator=g)  # noqa: E731
+    x, w = rand(g, (M, K), "bf16"), rand(g, (K, N), "bf16", K ** -0.5)
+    rows, t = [0, 65535, 65536, 65537, M - 1], torch.bfloat16
+    y = empty((M, N), "bf16")
+    print("linear", flush=True)
+    program(operators.linear, "bf16").launch([x, w, y])
+    want = x[rows].double() @ w.double()
+    close(y[rows], want, ref.product_bound(x[rows].double(), w.double()) + ref.half_step(t, want) + 1e-30, "y")
+    print("layer_norm", flush=True)
+    z, gamma, beta = big(), rand(g, (N,), "bf16", 0.3, 1.0), rand(g, (N,), "bf16", 0.5)
+    program(operators.layer_norm, "bf16").launch([z, gamma, beta, y], scalars=(EPS,))
+    args = [v.double() for v in (z[rows], gamma, beta)]
+    close(y[rows], ref.layer_norm(*args, EPS)[0], ref.layer_norm_bounds(*args, EPS, t)[0], "norm")
+    print("linear_backward", flush=True)
+    dy, dz, dx, dw = y.normal_(generator=g), empty((M, N), "bf16"), empty((M, K), "bf16"), empty((K, N), "bf16")
+    program(operators.linear_backward, "bf16", act="relu").launch([dy, x, w, z, dz, dx, dw])
+    assert torch.equal(dz[rows], torch.where(z[rows] > 0, dy[rows], torch.zeros_like(dy[rows])))
+    used = dz[rows].double()
+    want = used @ w.double().T
+    close(dx[rows], want, ref.product_bound(used, w.double().T) + ref.half_step(t, want) + 1e-30, "dx")
+    used = dz[:, N - 40:].double()
+    want = x.double().T @ used
+    close(dw[:, N - 40:], want, ref.product_bound(x.double().T, used) + ref.half_step(t, want) + 1e-30, "dw")
+
+
 def test_refusals_on_the_device(gpu):
     p = program(operators.linear, "bf16", bias=True, residual=True)
     t = lambda *s: torch.zeros(s, device="cuda", dtype=torch.bfloat16)  # noqa: E731

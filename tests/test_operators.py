@@ -82,7 +82,7 @@ def test_every_operator_is_listed_and_built():
     ("linear", "elem=f32", "elem=f32"), ("linear", "", "no elem"), ("linear", "elem=bf16 act=swish", "act=swish"),
     ("linear", "elem=bf16 stats", "stats"), ("linear", "elem=bf16 bias=1", "bias=1"), ("linear", "elem=bf16 elem=f16", "twice"),
     ("gated", "elem=bf16 residual", "residual"), ("gated_backward", "elem=bf16 save", "save"), ("linear", "elem=bf16 act", "act"),
-    ("layer_norm", "elem=bf16 act=gelu", "act=gelu"), ("layer_norm", "elem=bf16 weight=f16", "weight=f16"),
+    ("layer_norm", "elem=bf16 act=gelu", "act=gelu"), ("layer_norm", "elem=bf16 weight=f16", "weight=f16"), ("layer_norm", "elem=bf16 weight=elem", "weight=elem"),
     ("layer_norm", "elem=u8", "elem=u8"), ("linear_backward", "elem=bf16 residual", "residual")])
 def test_refused_attributes(op, attributes, word):
     with pytest.raises(BuildError, match=word):
