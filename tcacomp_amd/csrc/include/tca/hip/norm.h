@@ -6,6 +6,9 @@
 //             dx = s (t - sum_c t / C - h sum_c (t h) / C)  [+ dres]
 //             dgamma = sum_r dy h,  dbeta = sum_r dy
 //
+// The maps are chains of fused multiply-adds, so that a result is few roundings
+// away from its sums (-0 where there is nothing to add: it leaves -0 as it is).
+//
 // Both are bound by HBM: every operand is read once, every result written
 // once. A row is held in registers by a group of G lanes (16, a wave, or 4 or
 // 16 waves), NV vectors of 16 bytes a lane, so that the variance is the
@@ -141,8 +144,7 @@ __device__ __forceinline__ void norm_rows(const T* x, const W* __restrict__ gamm
       if constexpr (!HELD) weights(i);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        v[i][e] = v[i][e] * r * static_cast<float>(g[i][e]);
-        if constexpr (BIAS) v[i][e] += static_cast<float>(b[i][e]);
+        v[i][e] = __builtin_fmaf(v[i][e] * r, static_cast<float>(g[i][e]), BIAS ? static_cast<float>(b[i][e]) : -0.0f);
       }
       if (holds[i] == kNormAll) row_store<E, true, true>(y + row * C, (i * G + lane) * E, C, v[i]);
       else row_store<E, false, true>(y + row * C, (i * G + lane) * E, C, v[i]);
@@ -203,8 +205,7 @@ __device__ __forceinline__ void norm_long(const T* x, const W* __restrict__ gamm
     if constexpr (BIAS) row_load<E>(beta, c, C, b);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      v[e] = (v[e] - m) * r * g[e];
-      if constexpr (BIAS) v[e] += b[e];
+      v[e] = __builtin_fmaf((v[e] - m) * r, g[e], BIAS ? b[e] : -0.0f);
     }
     row_store<E>(yr, c, C, v);
   }
@@ -295,6 +296,7 @@ __device__ __forceinline__ void norm_backward_rows(const T* __restrict__ dy, con
     }
     norm_group_sums<G>(s, sums[turn & 1u]);
     if (!live) continue;
+    const float mt = s[0] * inv, mth = s[1] * inv;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (holds[i] == kNormNone) continue;
@@ -302,9 +304,8 @@ __device__ __forceinline__ void norm_backward_rows(const T* __restrict__ dy, con
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float h = (static_cast<float>(now.x[i][e]) - now.m) * now.rs;
-        const float t = static_cast<float>(now.dy[i][e]) * static_cast<float>(g[i][e]);
-        o[e] = (t - (s[0] + h * s[1]) * inv) * now.rs;
-        if constexpr (RES) o[e] += static_cast<float>(now.res[i][e]);
+        const float t = __builtin_fmaf(static_cast<float>(now.dy[i][e]), static_cast<float>(g[i][e]), -mt);
+        o[e] = __builtin_fmaf(__builtin_fmaf(-h, mth, t), now.rs, RES ? static_cast<float>(now.res[i][e]) : -0.0f);
       }
       if (holds[i] == kNormAll) row_store<E, true>(dx + row * C, (i * G + lane) * E, C, o);
       else row_store<E>(dx + row * C, (i * G + lane) * E, C, o);
@@ -357,8 +358,8 @@ __device__ __forceinline__ void norm_backward_long(const T* __restrict__ dy, con
   }
   float both[2] = {s1, s2};
   norm_group_sums<1024>(both, sums);
-  s1 = both[0];
-  s2 = both[1];
+  s1 = both[0] * inv;
+  s2 = both[1] * inv;
   for (uint32_t c = threadIdx.x * E; c < C; c += 1024u * E) {
     float h[E], t[E], g[E], o[E];
     row_load<E>(x + at, c, C, h);
@@ -367,8 +368,8 @@ __device__ __forceinline__ void norm_backward_long(const T* __restrict__ dy, con
     if constexpr (RES) row_load<E>(dres + at, c, C, o);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float d = (t[e] * g[e] - (s1 + (h[e] - m) * rs * s2) * inv) * rs;
-      o[e] = RES ? d + o[e] : d;
+      const float d = __builtin_fmaf(-(h[e] - m) * rs, s2, __builtin_fmaf(t[e], g[e], -s1));
+      o[e] = __builtin_fmaf(d, rs, RES ? o[e] : -0.0f);
     }
     row_store<E>(dx + at, c, C, o);
   }
