@@ -139,6 +139,7 @@ class Writer {
   struct Kernel {
     std::string suffix, params, body, grid, detail;  // params: tensor, dim and scalar names; grid: terms
     uint32_t block = 256;
+    uint32_t waves = 0;  // on a SIMD, that its registers have to leave room for
     std::vector<std::string> records;  // when, unless, split
     // Functions that stand in for it: their suffix, body and what they are, and
     // the plan's bounds (after "form <symbol>"); one may be listed again with others.
@@ -166,7 +167,8 @@ class Writer {
       }
     }
     auto function = [&](const std::string& name, const std::string& detail, const std::string& body) {
-      body_ << "// " << detail << "\nextern \"C\" __global__ void __launch_bounds__(" << k.block << ") " << name << "("
+      body_ << "// " << detail << "\nextern \"C\" __global__ void __launch_bounds__(" << k.block
+            << (k.waves != 0u ? ", " + std::to_string(k.waves) : "") << ") " << name << "("
             << sig << ") {\n" << body << "}\n\n";
     };
     function(symbol, k.detail, k.body);
@@ -521,6 +523,9 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   Writer::Kernel any;
   any.params = p.params;
   any.block = 512;
+  // Two workgroups a CU (4001 x 2049 x 3203 134 us with one, 112 so; what spills is
+  // read again outside the loop, but for rows of less than 8).
+  any.waves = 4;
   any.records = with(odd, {large_plane});
   if (p.pair) {  // 128 tiles and more
     any.suffix = p.suffix + "_a";

@@ -324,7 +324,7 @@ __device__ __forceinline__ u32x4 gather16(const uint16_t* p, uint32_t n) {
 // is loaded from 8 elements before that end and moved into place, so the tail
 // of k adds zeros. Slices first .. end - 1 of all segments'. Loads
 // of rows that start anywhere span a line more, and go through registers: half
-// the ring's rate (1001 x 1003 x 1501 16.2 us, 4001 x 2049 x 3203 99 us, 530 TFLOP/s).
+// the ring's rate (1001 x 1003 x 1501 15.0 us; 4001 x 2049 x 3203 112 us, with whole chunks 98).
 template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, typename Epi>
 __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& epi, uint32_t tile, uint32_t first, uint32_t end) {
   constexpr uint32_t HB = 64, THREADS = 512, SLICE = BM * 64u, HALF = HB * 64u, BUF = SLICE + 2u * HALF;
@@ -338,18 +338,22 @@ __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& 
   const uint32_t wm = (wave >> 2) * (BM / 2u), wn = (wave & 3u) * 16u;
 
   // One chunk of 8 of a K-contiguous panel row, or of row k of a row-contiguous
-  // panel, and its values in place.
-  auto kc_load = [&](const uint16_t* base, uint32_t row, uint32_t rows, uint32_t k) -> u32x4 {
+  // panel, and its values in place. TINY: rows of less than 8 values may occur,
+  // and are gathered; otherwise a load has no branch, so that the waits for the
+  // loads of one slice can leave those of the next in flight.
+  auto kc_load = [&](auto tiny, const uint16_t* base, uint32_t row, uint32_t rows, uint32_t k) -> u32x4 {
     const uint16_t* r = base + static_cast<uint64_t>(row < rows ? row : rows - 1u) * K;
-    if (K < 8u) return gather16(r + (k < K ? k : 0u), k < K ? K - k : 0u);
+    if constexpr (decltype(tiny)::value)
+      if (K < 8u) return gather16(r + (k < K ? k : 0u), k < K ? K - k : 0u);
     return load16_any(r + (k < K - 8u ? k : K - 8u));
   };
   auto kc_fix = [&](u32x4 v, uint32_t k) -> u32x4 {
     return K < 8u || k + 8u <= K ? v : shift_down16(v, k - (K - 8u));
   };
-  auto rc_load = [&](const uint16_t* base, uint32_t c, uint32_t cols, uint32_t k) -> u32x4 {
+  auto rc_load = [&](auto tiny, const uint16_t* base, uint32_t c, uint32_t cols, uint32_t k) -> u32x4 {
     const uint16_t* r = base + static_cast<uint64_t>(k < K ? k : K - 1u) * cols;
-    if (cols < 8u) return gather16(r + (c < cols ? c : 0u), c < cols ? cols - c : 0u);
+    if constexpr (decltype(tiny)::value)
+      if (cols < 8u) return gather16(r + (c < cols ? c : 0u), c < cols ? cols - c : 0u);
     return load16_any(r + (c < cols - 8u ? c : cols - 8u));
   };
   auto rc_fix = [&](u32x4 v, uint32_t c, uint32_t cols, uint32_t k) -> u32x4 {
@@ -363,19 +367,21 @@ __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& 
   };
   Regs regs[2];
   const uint32_t ns = (K + 63u) / 64u;
-  auto load = [&](Regs& r, uint32_t t) {
+  // Slice t, past the last one that again: every slice issues the same loads.
+  auto load = [&](auto tiny, Regs& r, uint32_t at) {
+    const uint32_t t = at < end ? at : end - 1u;
     const uint32_t seg = SEGS == 1 || t < ns ? 0u : 1u, k0 = (t - seg * ns) * 64u;
     const uint16_t* a = seg == 0u ? p.a[0] : p.a[SEGS - 1];
 #pragma unroll
     for (uint32_t i = 0; i < CA; ++i) {
       const uint32_t c = i * THREADS + tid;
-      r.a[i] = A_RC ? rc_load(a, m0 + c % kAC * 8u, M, k0 + c / kAC) : kc_load(a, m0 + (c >> 3), M, k0 + (c & 7u) * 8u);
+      r.a[i] = A_RC ? rc_load(tiny, a, m0 + c % kAC * 8u, M, k0 + c / kAC) : kc_load(tiny, a, m0 + (c >> 3), M, k0 + (c & 7u) * 8u);
     }
 #pragma unroll
     for (uint32_t h = 0; h < 2u; ++h) {
       const uint32_t hp = PAIR ? h : 0u, nh = PAIR ? n0 : n0 + HB * h;
       const uint16_t* b = seg == 0u ? p.b[hp][0] : p.b[hp][SEGS - 1];
-      r.b[h] = B_RC ? rc_load(b, nh + (tid & 7u) * 8u, N, k0 + (tid >> 3)) : kc_load(b, nh + (tid >> 3), N, k0 + (tid & 7u) * 8u);
+      r.b[h] = B_RC ? rc_load(tiny, b, nh + (tid & 7u) * 8u, N, k0 + (tid >> 3)) : kc_load(tiny, b, nh + (tid >> 3), N, k0 + (tid & 7u) * 8u);
     }
   };
   auto write = [&](Regs& r, uint32_t t, uint32_t buf) {
@@ -436,24 +442,39 @@ __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& 
         for (int i = 0; i < IM; ++i) acc[i][h] = mfma_16x16x32_16b<F16>(fb[h], fa[i], acc[i][h]);
     }
   };
-  if (first < end) {
-    load(regs[0], first);
-    if (first + 1u < end) load(regs[1], first + 1u);
+  auto run = [&](auto tiny) {
+    auto fence = []() { __builtin_amdgcn_sched_barrier(0); };  // loads stay in the order that the waits count
+    load(tiny, regs[0], first);
+    fence();
+    load(tiny, regs[1], first + 1u);
+    fence();
     write(regs[0], first, 0u);
-    if (first + 2u < end) load(regs[0], first + 2u);
+    fence();
+    load(tiny, regs[0], first + 2u);
+    fence();
     __syncthreads();
-    for (uint32_t t = first; t < end; t += 2u) {
-#pragma unroll
-      for (uint32_t i = 0; i < 2u; ++i) {  // slice t + i, in buffer i; the next one in the registers of its parity
-        const uint32_t s = t + i;
-        if (s < end) {
-          compute(i);
-          if (s + 1u < end) write(regs[1u - i], s + 1u, 1u - i);
-          if (s + 3u < end) load(regs[1u - i], s + 3u);
-          __syncthreads();
-        }
-      }
+    // Slice t, in buffer i; the next one (past the last: that again, read by
+    // no one) in the registers of its parity.
+    auto slice = [&](uint32_t t, uint32_t i) {
+      compute(i);
+      write(regs[1u - i], t + 1u < end ? t + 1u : t, 1u - i);
+      load(tiny, regs[1u - i], t + 3u);
+      __syncthreads();
+    };
+    // (Whole pairs: a way out between the two would make every wait one for all loads.)
+    uint32_t t = first;
+    for (; t + 2u <= end; t += 2u) {
+      slice(t, 0u);
+      slice(t + 1u, 1u);
     }
+    if (t < end) {
+      compute(0u);
+      __syncthreads();
+    }
+  };
+  if (first < end) {
+    if ((A_RC ? M : K) < 8u || (B_RC ? N : K) < 8u) run(std::true_type{});
+    else run(std::false_type{});
   }
   // (the last slice's barrier: no wave reads the slices any more)
   product_store<IM, 1, PAIR, false>(acc, reinterpret_cast<float*>(lds) + wave * (32u * (IM < 4 ? 16u * IM : 64u)), m0 + wm, n0 + wn, HB, M, N,
