@@ -374,8 +374,8 @@ constexpr uint32_t kFewRows = 64;
 // Workgroups that products of few tiles are split into, by k: as many as CUs.
 constexpr uint32_t kCUs = 256;
 // Planes of at most so many results may be split (64 tiles of 128x128: into four and
-// more; two parts pay for the sum of their halves what they save: dx of 2048 x
-// 1024 x 4096, 128 tiles, 31 us in one launch, 25 and 5 in two parts).
+// more; two parts pay for the sum of their halves more than they save: dx of 2048 x
+// 1024 x 4096, 128 tiles, 25 and 5 us in two parts, 25 in one of half the tile).
 constexpr uint64_t kSplitPlane = 1ull << 20;
 
 void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
@@ -485,12 +485,13 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   };
   few_tiles("_k", "product_ring<" + targs + ", 128, 64, 2, 2, 5, 5>", 256, 128, aligned, "tiles of 128x128, direct to LDS");
   Writer::Kernel k;
-  k.suffix = p.suffix + "_r";
+  const std::string cfg_r = "product_ring<" + targs + ", 128, 64, 2, 2, 5, 5>";
+  k.suffix = p.suffix + (p.pair ? "_r" : "_t");
   k.params = p.params;
   k.records = with(aligned, {large_plane});
-  k.body = body("product_ring<" + targs + ", 128, 64, 2, 2, 5, 5>");
-  k.grid = tiles(128, 128);
-  k.detail = p.what + ", tiles of 128x128 (256x256, 256x128 where they fill the card), 4 waves, direct to LDS";
+  k.body = body(p.pair ? cfg_r : "product_ring<" + targs + ", 64, 64, 2, 2, 5, 5>");
+  k.grid = p.pair ? tiles(128, 128) : tiles(64, 128);
+  k.detail = p.what + (p.pair ? ", tiles of 128x128" : ", tiles of 64x128") + " (up to 256x256 where they fill the card), 4 waves, direct to LDS";
   // Larger tiles load less for a product, and need more of the plane to fill
   // 256 CUs; one workgroup of 256x256 or 256x128 holds a CU, two of 128x128 with
   // shorter rings do. Bounds by whole rounds of the card, at k = 4096 (us, bf16, _l /
@@ -500,6 +501,8 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   //                       96: 82.5 / 53.2 / 53.5 / 64.5   256: 104 / 118 / 121 / 145
   //                      272: 172 / 155 / 167 / 188       384: 191 / 179 / 202 / 244
   //                      400: 187 / 217 / 236 / 274       512: 203 / 242 / 263 / 310
+  // Up to 128 tiles of 128x128, tiles of 64x128 put a workgroup on twice as many
+  // CUs (_r / 64x128: 2048 x 1024 30.7 / 25.3; 1536 x 1664, 156 tiles, 31.0 / 45.5).
   auto form = [&](Writer::Kernel* of, const char* suffix, const std::string& what, const std::string& call, uint32_t rows,
                   uint32_t cols, uint32_t least, const std::string& terms) {
     // its grid, then the bound: at least so many tiles, of `terms`
@@ -515,6 +518,7 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   form(&k, "_l", what_l, cfg_l, 256, 256, 257, tall);
   form(&k, "_m", what_m, cfg_m, 256, 128, 192, tall);
   form(&k, "_s", what_s, cfg_s, 128, 128, 257, small);
+  if (!p.pair) form(&k, "_r", "tiles of 128x128, one workgroup a CU", cfg_r, 128, 128, 129, small);
   w->Add(k);
   // (1101 x 1001 x 2049, 72 tiles of 128x128: 34 us, of 64x128 27; 132 of them 35 and
   // 36; 432, 53 and 70.)

@@ -344,7 +344,7 @@ def test_gated_backward_attributes(gpu, M, K, N, elem, attrs):
 
 
 @pytest.mark.parametrize("M,K,N", [(3592, 72, 3608), (3592, 264, 3600), (2056, 72, 3080), (1032, 40, 3080), (1504, 72, 2904),
-                                   (1000, 40, 2304)])
+                                   (1000, 40, 2304), (1032, 72, 1608)])
 def test_large_planes(gpu, M, K, N):
     """Planes of many tiles, their last row and column of tiles partial, a
     reduction that ends inside a slice."""

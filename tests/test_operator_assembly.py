@@ -140,7 +140,7 @@ def test_matrix_instructions_and_their_hazards(rings):
     for name, (_, code) in rings.items():
         flow = Flow(code)
         mfma = [i for i, l in enumerate(code) if l.startswith("v_mfma")]
-        assert len(mfma) >= 64, name
+        assert len(mfma) >= 32, name
         for i in mfma:
             ops = [o.strip() for o in code[i].split(None, 1)[1].split(",")]
             assert ops[0] == ops[3] and ops[0].startswith("a["), code[i]

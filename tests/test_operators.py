@@ -175,10 +175,10 @@ def product_kernels(M, N, K, few, odd, half=1):
         return {"_a": tiles(128, 128)} if tiles(128, 128) >= 128 else {"": tiles(64, 128)}
     for form, rows, cols, least, of in (("_l", 256, 256, 385, (256, 256)), ("_m", 256, 128, 257, (256, 256)),
                                         ("_l", 256, 256, 257, (256, 128)), ("_m", 256, 128, 192, (256, 128)),
-                                        ("_s", 128, 128, 257, (128, 128))):
+                                        ("_s", 128, 128, 257, (128, 128)), ("_r", 128, 128, 129, (128, 128))):
         if tiles(*of) >= least:
             return {form: tiles(rows, cols)}
-    return {"_r": tiles(128, 128)}
+    return {"_r": tiles(128, 128)} if half == 2 else {"_t": tiles(64, 128)}
 
 
 def launched(p, plan, tensors, dims):
