@@ -109,6 +109,17 @@ def product_bound(a, b):
     return 1e-5 * math.sqrt(K) * a.norm(dim=1)[:, None] * b.norm(dim=0)[None, :]
 
 
+def walk_bound(a, b):
+    """|error| of the same sum where a and b are random of mean zero: the
+    rounding errors of at most K + 64 additions (k, and the joins of waves and
+    parts), each within a step, 2 U, of the partial sum there, add as a random
+    walk. A partial sum is of the size of sqrt(sum a^2 b^2) or, on the way to a
+    far result, of the result; eight deviations (Azuma: 2 exp(-32) an element).
+    It is below what a partial sum rounded to 16 bits is off by."""
+    K = max(1, a.shape[1])
+    return 16 * U * math.sqrt(K + 64) * (((a * a) @ (b * b)).sqrt() + (a @ b).abs())
+
+
 def act_error(z):
     """Relative error of an activation's or slope's terms in f32: the argument
     of exp or erfc carries a rounding of z^2 or z^3 (gelu_tanh: 1.6 z (1 +
