@@ -140,7 +140,7 @@ class Writer {
     std::string suffix, params, body, grid, detail;  // params: tensor, dim and scalar names; grid: terms
     uint32_t block = 256;
     uint32_t waves = 0;  // on a SIMD, that its registers have to leave room for
-    std::vector<std::string> records;  // when, unless, split
+    std::vector<std::string> records;  // when, unless, split, scratch
     // Functions that stand in for it: their suffix, body and what they are, and
     // the plan's bounds (after "form <symbol>"); one may be listed again with others.
     struct Form {
@@ -209,6 +209,13 @@ std::string When(const std::string& dims, uint64_t lo, uint64_t hi, uint64_t mod
   return "when " + dims + " " + std::to_string(lo) + " " + std::to_string(hi) + " " + std::to_string(mod) + " 0";
 }
 constexpr uint64_t kMost = 4294967295ull;
+// What a kernel writes of local `tensor`, as grid terms.
+std::string Scratch(const std::string& tensor, const std::string& terms) {
+  int n = 0;
+  std::istringstream in(terms);
+  for (std::string t; in >> t;) ++n;
+  return "scratch " + tensor + " " + std::to_string(n) + " " + terms;
+}
 
 // ------------------------------------------------------------- layer norm
 
@@ -275,8 +282,8 @@ void EmitLayerNormBackward(const Attrs& a, Writer* w) {
   w->Header("tca/hip/norm.h");
   w->Dim("R");
   w->Dim("C");
-  // Partial rows of the weights' gradients: at most 32 MiB of them for rows
-  // in registers, as many as a launch that allocates nothing may use.
+  // Partial rows of the weights' gradients: at most 16 MiB of them for rows
+  // in registers (8192 values by two gradients).
   const uint32_t kParts = 256, kLongParts = 32;
   w->Dim("parts", kParts);
   w->Dim("long_parts", kLongParts);
@@ -297,6 +304,9 @@ void EmitLayerNormBackward(const Attrs& a, Writer* w) {
   const std::string args = "(dy, x, gamma, mean, rstd, " + (res ? "dres" : none) + ", dx, ";
   const uint32_t E = a.elem == "f32" ? 4u : 8u;
   uint64_t from = 0;
+  auto scratch = [&](const std::string& part, uint32_t groups, uint32_t most) {
+    return Scratch(part, "R/" + std::to_string(groups) + ":" + std::to_string(most) + " C/1" + (bias ? " 2/1" : ""));
+  };
   auto join = [&](const std::string& suffix, const std::string& part, uint32_t groups, uint32_t most, uint64_t lo, uint64_t hi) {
     Writer::Kernel j;
     j.suffix = suffix;
@@ -322,7 +332,7 @@ void EmitLayerNormBackward(const Attrs& a, Writer* w) {
     k.body = "  tca::hip::norm_backward_rows<" + T + ", " + W + ", " + g + ", " + v + ", " + Bool(bias) + ", " + Bool(res) +
              ">" + args + "part, R, C);\n";
     k.grid = "R/" + std::to_string(groups) + ":" + std::to_string(kParts);
-    k.records = {When("C", from, to)};
+    k.records = {When("C", from, to), scratch("part", groups, kParts)};
     k.detail = "rows of " + std::to_string(from) + " to " + std::to_string(to) + " in registers, " + g + " lanes of " + v +
                " vectors, partial weight gradients";
     w->Add(k);
@@ -344,7 +354,7 @@ void EmitLayerNormBackward(const Attrs& a, Writer* w) {
   const std::string parts = "tca::hip::partial_rows(R, 64u, " + std::to_string(kLongParts) + "u)";
   c.body = "  tca::hip::norm_backward_columns<" + T + ", " + Bool(bias) + ">(dy, x, mean, rstd, long_part, R, C, " + parts + ");\n";
   c.grid = "C/" + std::to_string(64u * E) + " R/64:" + std::to_string(kLongParts);
-  c.records = {When("C", from, kMost)};
+  c.records = {When("C", from, kMost), scratch("long_part", 64, kLongParts)};
   c.detail = "partial weight gradients of rows from " + std::to_string(from) + " on, by columns";
   w->Add(c);
   join("_long_join", "long_part", 64, kLongParts, from, kMost);
@@ -390,6 +400,7 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   const std::string f16 = Bool(a.elem == "f16"), pair = Bool(p.pair);
   const std::string targs = f16 + ", " + Bool(p.a_rc) + ", " + Bool(p.b_rc) + ", " + pair + ", " + std::to_string(p.segs);
   const std::string plane = p.M + "*" + p.N, part = "part";
+  const std::string sums = Scratch(part, plane + "/1" + (p.pair ? " 2/1" : ""));  // of each of P parts
   // Tiles of rows x cols (of a pair: cols / 2 of each product) as grid terms, and counted on the device.
   auto tiles = [&](uint32_t rows, uint32_t cols) {
     return p.M + "/" + std::to_string(rows) + " " + p.N + "/" + std::to_string(p.pair ? cols / 2u : cols);
@@ -442,7 +453,7 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
       k.body = ops.str() + "  tca::hip::product_few<" + f16 + ", " + pair + ", " + std::to_string(blocks) + ">(p, epi, " + part + ", " +
                strips + ", " + P + ");\n";
       k.grid = terms;
-      k.records = {split(least, terms, "0"), When("M", from, 16u * blocks)};
+      k.records = {split(least, terms, "0"), sums, When("M", from, 16u * blocks)};
       k.detail = p.what + ", " + std::to_string(from) + " to " + std::to_string(16u * blocks) + " rows, strips of 64 columns, k over 8 waves and P workgroups";
       w->Add(k);
       from = 16u * blocks + 1u;
@@ -478,7 +489,7 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
              std::to_string(p.segs) + "u, chunk, P);\n  tca::hip::" + call + "(p, tca::hip::split_store<" + pair + ">(epi, " + part +
              ", chunk, P, p.M, p.N), blockIdx.x % tiles, run.first, run.end);\n";
     k.grid = terms;
-    k.records = with(records, {split(least, terms, "0"), small_plane});
+    k.records = with(records, {split(least, terms, "0"), sums, small_plane});
     k.detail = p.what + ", " + detail + ", k over P workgroups (at most " + std::to_string(kSplitPlane) + " results)";
     w->Add(k);
     join(suffix + "join", 4, P, split(least, terms, "1"), with(records, {small_plane}), detail);
@@ -631,6 +642,8 @@ void EmitBackward(const Attrs& a, bool gated, Writer* w) {
     k.block = 1024;
     k.body = f + "  tca::hip::slope_columns(f, bias_part, M, N, " + parts + ");\n";
     k.grid = "N/512 M/" + std::to_string(kPartRows) + ":" + std::to_string(kParts);
+    k.records = {Scratch("bias_part", "M/" + std::to_string(kPartRows) + ":" + std::to_string(kParts) + " N/1" +
+                                          (gated ? " 2/1" : ""))};
     k.detail = "gradients of the pre-activations, partial sums of the bias' gradient";
     w->Add(k);
     Writer::Kernel j;

@@ -246,6 +246,22 @@ bool Parse(const std::string& text, Plan* out, std::string* err) {
         if (t.packed) return bad("a split term cannot divide by 'pack'");
         k.split_terms.push_back(t);
       }
+    } else if (kw == "scratch") {
+      if (p.kernels.empty()) return bad("scratch before any kernel");
+      Kernel::Scratch s;
+      uint64_t nt = 0;
+      if (tok.size() < 3 || !ParseU64(tok[2], &nt) || tok.size() != 3 + nt || nt == 0)
+        return bad("scratch <tensor> <n-terms> <term>...");
+      s.tensor = FindTensor(p, tok[1]);
+      if (s.tensor < 0 || p.tensors[s.tensor].role != Role::Local) return bad("scratch names no local " + tok[1]);
+      for (uint64_t i = 0; i < nt; ++i) {
+        Term t;
+        std::string e;
+        if (!ParseTerm(p, tok[3 + i], &t, &e)) return bad(e);
+        if (t.packed) return bad("a scratch term cannot divide by 'pack'");
+        s.terms.push_back(t);
+      }
+      p.kernels.back().scratch.push_back(s);
     } else if (kw == "stride") {
       if (p.kernels.empty()) return bad("stride before any kernel");
       if (tok.size() != 2 || !ParseU64(tok[1], &p.kernels.back().stride) || p.kernels.back().stride == 0)
@@ -399,6 +415,11 @@ std::string Serialize(const Plan& p) {
       for (const auto& t : k.split_terms) o << " " << TermText(p, t);
       o << "\n";
     }
+    for (const auto& s : k.scratch) {
+      o << "scratch " << p.tensors[s.tensor].name << " " << s.terms.size();
+      for (const auto& t : s.terms) o << " " << TermText(p, t);
+      o << "\n";
+    }
     if (k.stride != 0) o << "stride " << k.stride << "\n";
     for (const auto& f : k.forms) {
       o << "form " << f.symbol << " " << f.stride << " " << f.bounds.size();
@@ -516,26 +537,52 @@ int Bind(const Plan& p, const tca_tensor* tensors, uint32_t n_tensors, const uin
 }
 
 bool WorkspaceLayout(const Plan& p, const std::vector<uint32_t>& dims, const std::vector<bool>& used,
-                     std::vector<size_t>* off, size_t* total, std::string* err) {
+                     std::vector<size_t>* off, size_t* total, size_t* bound, std::string* err) {
   constexpr size_t kMax = std::numeric_limits<size_t>::max();
   off->assign(p.tensors.size(), 0);
-  *total = 0;
+  *total = *bound = 0;
+  // n *= x, false where that does not fit.
+  auto times = [](size_t* n, uint64_t x) {
+    if (x != 0 && *n > kMax / x) return false;
+    *n *= x;
+    return true;
+  };
   for (size_t t = 0; t < p.tensors.size(); ++t) {
     if (p.tensors[t].role != Role::Local || !used[t]) continue;
-    size_t n = DtypeBytes(p.tensors[t].dtype);
-    for (int d : p.tensors[t].dims) {
-      if (dims[d] != 0 && n > kMax / dims[d]) {
-        *err = "program " + p.name + ": local " + p.tensors[t].name + " exceeds the address space at these dims";
-        return false;
+    const size_t bytes = DtypeBytes(p.tensors[t].dtype);
+    size_t declared = bytes, written = 0;
+    bool fits = true, records = false;
+    for (int d : p.tensors[t].dims) fits = fits && times(&declared, dims[d]);
+    for (const auto& k : p.kernels) {
+      if (k.scratch.empty() || !Selected(k, dims)) continue;
+      const uint64_t chunks = SplitChunks(k, dims);
+      for (const auto& s : k.scratch) {
+        if (s.tensor != static_cast<int>(t)) continue;
+        records = true;
+        if (k.split_dim >= 0 && chunks == 1) continue;
+        size_t n = bytes;
+        bool overflow = false;
+        fits = fits && times(&n, chunks);
+        for (const auto& term : s.terms) fits = fits && times(&n, TermValue(k, term, dims, &overflow));
+        fits = fits && !overflow;
+        written = std::max(written, n);
       }
-      n *= dims[d];
     }
-    if (n > kMax - 255u || *total > kMax - ((n + 255u) & ~static_cast<size_t>(255u))) {
+    if (!fits) {
+      *err = "program " + p.name + ": local " + p.tensors[t].name + " exceeds the address space at these dims";
+      return false;
+    }
+    const size_t need = records ? written : declared, most = std::max(need, declared);
+    auto add = [](size_t* sum, size_t n) {
+      if (n > kMax - 255u || *sum > kMax - ((n + 255u) & ~static_cast<size_t>(255u))) return false;
+      *sum += (n + 255u) & ~static_cast<size_t>(255u);
+      return true;
+    };
+    (*off)[t] = *total;
+    if (!add(total, need) || !add(bound, most)) {
       *err = "program " + p.name + ": workspace exceeds the address space at these dims";
       return false;
     }
-    (*off)[t] = *total;
-    *total += (n + 255u) & ~static_cast<size_t>(255u);
   }
   return true;
 }

@@ -25,6 +25,11 @@
 //       partials) launches only when P > 1; mode 2: the kernel launches only
 //       when P == 1 (a whole-column kernel); mode 3: as mode 0, but only when
 //       P > 1 (the partials of a nest whose P == 1 case is a mode-2 kernel).
+//   scratch <tensor> <n-terms> <term>...    (for the last kernel) the kernel writes
+//       at most the product of the terms elements of local <tensor>; with a
+//       split record P times that, and nothing where P is 1. A local that
+//       kernels running at these dims have such records of needs the largest of
+//       them, in place of its declared extents, which bound it.
 //   stride <n>    (for the last kernel) the kernel walks its work with the
 //       grid as its stride: at most n workgroups are launched
 //   form <symbol> <stride> <n> <min> <n-terms> <term>... ...    (for the last
@@ -136,6 +141,12 @@ struct Kernel {
   // only when P == 1, kSplitPartialMany = grid x P, launched only when P > 1.
   int split_mode = 0;
   std::vector<Term> split_terms;
+  // What it writes of a local (see the scratch record).
+  struct Scratch {
+    int tensor = 0;
+    std::vector<Term> terms;
+  };
+  std::vector<Scratch> scratch;
   uint64_t stride = 0;  // > 0: the most workgroups launched (a grid-stride kernel)
   std::vector<Form> forms;
 };
@@ -174,9 +185,11 @@ int Bind(const Plan& p, const tca_tensor* tensors, uint32_t n_tensors, const uin
 
 // The workspace at bound dims: every local that `used` marks at a 256-byte
 // aligned offset, in declaration order (`off` per plan tensor, `total` the
-// bytes). False, with `err` set, when a size does not fit in size_t.
+// bytes; `bound` the bytes with every one of them at its declared extents, or
+// `total` if that is more). False, with `err` set, when a size does not fit in
+// size_t.
 bool WorkspaceLayout(const Plan& p, const std::vector<uint32_t>& dims, const std::vector<bool>& used,
-                     std::vector<size_t>* off, size_t* total, std::string* err);
+                     std::vector<size_t>* off, size_t* total, size_t* bound, std::string* err);
 bool GridSize(const Kernel& k, const Plan& p, const std::vector<uint32_t>& dims, uint64_t* grid, std::string* err);
 // Rows per block of a packed kernel (1 otherwise); *block receives the
 // launch block size.

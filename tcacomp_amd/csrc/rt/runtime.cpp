@@ -123,7 +123,10 @@ struct tca_program_s {
     std::vector<uint8_t> nonempty;    // per tensor parameter: it has elements (data must be valid)
     std::vector<int> param_of;        // per plan tensor: its parameter index, -1 for a local
     std::vector<size_t> local_off;    // per plan tensor: offset of a local in the workspace
-    size_t ws_bytes = 0;
+    // What the kernels use of the workspace at these dims, and what is allocated
+    // for it: the locals at their declared extents, so that a launch at other
+    // dims, a captured one too, mostly finds room.
+    size_t ws_bytes = 0, ws_bound = 0;
     struct Launch {
       hipFunction_t fn = nullptr;
       uint32_t grid = 0, block = 0, lds = 0;
@@ -510,7 +513,7 @@ int prepare_launch(tca_program p, const tca_tensor* tensors, uint32_t n_tensors,
     for (const auto& a : k.args)
       if (a.kind == tca::plan::ArgKind::Ptr) used[a.index] = true;
   }
-  if (!tca::plan::WorkspaceLayout(pl, dims, used, &pr->local_off, &pr->ws_bytes, &err))
+  if (!tca::plan::WorkspaceLayout(pl, dims, used, &pr->local_off, &pr->ws_bytes, &pr->ws_bound, &err))
     return fail(TCA_ERR_INVALID, "%s", err.c_str());
   pr->param_of.assign(pl.tensors.size(), -1);
   int next_param = 0;
@@ -622,11 +625,11 @@ int launch_program(tca_program p, const tca_tensor* tensors, uint32_t n_tensors,
     ws = tca::rt::ScratchPtr(dev);
     if (ws == nullptr)
       return fail(TCA_ERR_INVALID, "program_launch_noalloc: tca_rt_init(%d) has not set up this device", dev);
-  } else if (pr->ws_bytes > 0) {
+  } else if (pr->ws_bound > 0 && !noalloc) {
     lk.lock();
     tca_program_s::Workspace& w = p->workspaces[stream];
     const bool capturing = is_capturing(stream);
-    if (w.bytes < pr->ws_bytes) {
+    if (w.bytes < (capturing ? pr->ws_bytes : pr->ws_bound)) {
       // An allocation would end the capture; nothing has been queued yet.
       if (capturing)
         return fail(TCA_ERR_INVALID,
@@ -644,10 +647,10 @@ int launch_program(tca_program p, const tca_tensor* tensors, uint32_t n_tensors,
         w.ptr = nullptr;
         w.bytes = 0;
       }
-      TCA_HIP_TRY(hipMalloc(&w.ptr, pr->ws_bytes));
-      w.bytes = pr->ws_bytes;
+      TCA_HIP_TRY(hipMalloc(&w.ptr, pr->ws_bound));
+      w.bytes = pr->ws_bound;
     }
-    w.captured |= capturing;
+    w.captured |= capturing && pr->ws_bytes > 0;
     ws = w.ptr;
   }
 
@@ -717,8 +720,8 @@ int tca_program_kernel_args(tca_program p, const tca_tensor* tensors, uint32_t n
   }
   std::vector<size_t> local_off;
   std::vector<int> param_of(pl.tensors.size(), -1);
-  size_t ws_bytes = 0;
-  if (!tca::plan::WorkspaceLayout(pl, dims, used, &local_off, &ws_bytes, &err))
+  size_t ws_bytes = 0, ws_bound = 0;
+  if (!tca::plan::WorkspaceLayout(pl, dims, used, &local_off, &ws_bytes, &ws_bound, &err))
     return fail(TCA_ERR_INVALID, "%s", err.c_str());
   int next_param = 0;
   for (size_t t = 0; t < pl.tensors.size(); ++t)
