@@ -158,7 +158,10 @@ int tca_program_selected(tca_program p, const tca_tensor* tensors, uint32_t n_te
  * synchronizes the stream before it replaces the buffer). The first launch
  * that needs a workspace allocates (hipMalloc), so it cannot be captured
  * into a HIP graph: on a stream that is being captured, a launch that would
- * have to allocate fails with TCA_ERR_INVALID before anything is queued. A
+ * have to allocate fails with TCA_ERR_INVALID before anything is queued, in
+ * every capture mode (HIP does not tell a capture's mode, and in any but the
+ * relaxed one the allocation ends the capture). Launch once at the dims, and
+ * on the stream, that will be captured, or use tca_program_launch_noalloc. A
  * workspace that a captured launch uses is kept until unload, also when a
  * larger launch outgrows it. Graphs captured on one stream share its
  * workspace as the launches on it do: replay them in turn. */

@@ -184,6 +184,30 @@ def test_noalloc_launch_of_few_tokens(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["global", "thread_local", "relaxed"])
+def test_a_refused_launch_leaves_the_capture(gpu, mode):
+    """A launch that would allocate while its stream is captured, also after one
+    on another stream: refused in every mode, and the capture goes on, with the
+    allocation-free launch in its place."""
+    g = gen_of("refused")
+    p = compiler.compile_program(operators.linear("bf16"))
+    M, K, N = 5, 1000, 90
+    x, w, y, want = rand(g, (M, K), "bf16"), rand(g, (K, N), "bf16"), empty((M, N), "bf16"), empty((M, N), "bf16")
+    p.launch([x, w, want])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream(), capture_error_mode=mode):
+        with pytest.raises(_lib.TcaError, match="being captured"):
+            p.launch([x, w, y])
+        p.launch([x, w, y], noalloc=True)
+    for _ in range(3):
+        y.fill_(-1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
 def test_a_launch_that_needs_no_workspace_is_captured_at_once(gpu):
     """K in one part writes no partial sums: a first launch may be captured, and
     replayed between eager launches."""
