@@ -259,7 +259,9 @@ void EmitLayerNorm(const Attrs& a, Writer* w) {
     k.params = params;
     k.block = block;
     k.body = "  tca::hip::norm_rows<" + T + ", " + W + ", " + g + ", " + v + tail;
-    // as many workgroups as the card holds at once, at most
+    // At most 2048 lanes a CU, eight waves a SIMD. The narrow forms fit so; 64x4 (93
+    // VGPRs in f32, 141 in f16) has five and three waves resident and 256x4 (115,
+    // 188) four and two: their workgroups come in two to four rounds.
     k.grid = "R/" + std::to_string(block / f.lanes) + ":" + std::to_string(kLanes / block);
     k.records = {When("C", from, to)};
     k.detail = "rows of " + std::to_string(from) + " to " + std::to_string(to) + " in registers, " + g + " lanes of " + v + " vectors";
@@ -538,8 +540,9 @@ void EmitProduct(const Attrs& a, const Product& p, Writer* w) {
   Writer::Kernel any;
   any.params = p.params;
   any.block = 512;
-  // Two workgroups a CU (4001 x 2049 x 3203 134 us with one, 112 so; what spills is
-  // read again outside the loop, but for rows of less than 8).
+  // Two workgroups a CU (bf16 4001 x 2049 x 3203 111 us with one, 97 so; 1501 x 1003 x
+  // 1701, 168 tiles, 19 either way; what spills is read again outside
+  // the loop, but for rows of less than 8).
   any.waves = 4;
   any.records = with(odd, {large_plane});
   if (p.pair) {  // 128 tiles and more

@@ -23,10 +23,10 @@
 // in the same order.
 //
 // Measured: forward f32 [32768, 1024] with the statistics 46 to 48 us (268 MB, 5.6 to
-// 5.8 TB/s), f16 [3000, 8000] 24, [1618, 16880] 31; backward bf16 [8192, 4096]
-// with a residual 43 to 45 us (268 MB, 6.0 TB/s) and 4 to 5 for the join. Streaming
-// stores (forward) and loads (backward) took 5 and 8% off, loads a row ahead
-// and joins of 1024 lanes 10 and 30%.
+// 5.8 TB/s), bf16 [16384, 4096] 51, f16 [3000, 8000] 24, [1618, 16880] 29; backward
+// bf16 [8192, 4096] with a residual 43 to 45 us (268 MB, 6.0 TB/s) and 4 to 5 for
+// the join. Streaming stores (forward) and loads (backward) took 5 and 8% off,
+// loads a row ahead and joins of 1024 lanes 10 and 30%.
 #ifndef TCA_HIP_NORM_H_
 #define TCA_HIP_NORM_H_
 

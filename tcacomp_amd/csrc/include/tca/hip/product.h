@@ -323,8 +323,9 @@ __device__ __forceinline__ u32x4 gather16(const uint16_t* p, uint32_t n) {
 // (two buffers, one barrier a slice). A chunk that runs past the end of its row
 // is loaded from 8 elements before that end and moved into place, so the tail
 // of k adds zeros. Slices first .. end - 1 of all segments'. Loads
-// of rows that start anywhere span a line more, and go through registers: half
-// the ring's rate (1001 x 1003 x 1501 15.0 us; 4001 x 2049 x 3203 112 us, with whole chunks 98).
+// of rows that start anywhere span a line more, and go through registers: about
+// half the ring's rate (bf16 4001 x 2049 x 3203 97 us; 4000 x 2048 x 3200 in the ring
+// 54. f16 1001 x 1003 x 1501 with gelu, saved, 15.0).
 template <bool F16, bool A_RC, bool B_RC, bool PAIR, int SEGS, uint32_t BM, typename Epi>
 __device__ __forceinline__ void product_any(const Operands<SEGS>& p, const Epi& epi, uint32_t tile, uint32_t first, uint32_t end) {
   constexpr uint32_t HB = 64, THREADS = 512, SLICE = BM * 64u, HALF = HB * 64u, BUF = SLICE + 2u * HALF;
