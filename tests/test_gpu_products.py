@@ -69,3 +69,24 @@ def test_gradients_repeat_bit_for_bit(gpu):
             runs.append([base.empty(s, elem) for s in ((M, N), (M, K), (K, N), (N,))])
             p.launch([dy, x, w, z] + runs[-1])
         assert all(torch.equal(a, b) for r in runs for a, b in zip(runs[0], r))
+
+
+@pytest.mark.parametrize("M,K,N", [(70, 0, 91), (3, 0, 21), (0, 41, 63), (30, 0, 63), (30, 41, 0), (1200, 0, 1000), (0, 1200, 1000),
+                                   (1101, 0, 1001), (0, 1101, 1001), (1200, 1000, 0), (1101, 1001, 0)])
+def test_empty_extents(gpu, M, K, N):
+    """No reduction leaves the bias and the residual, no tokens zero gradients of
+    the weights, in every kind of kernel."""
+    print("empty", M, K, N, flush=True)
+    base.check_linear("bf16", M, K, N, bias=True, residual=True)
+    base.check_gated("f16", M, K, N, act="gelu", bias=True, save=True)
+    base.check_linear_backward("bf16", M, K, N, act="gelu", bias=True)
+    base.check_gated_backward("f16", M, K, N)
+
+
+@pytest.mark.parametrize("M,K,N", [(20000, 24, 40), (9001, 17, 1027)])
+def test_bias_gradients_of_many_rows(gpu, M, K, N):
+    """More than 16 rows a partial row of the bias' gradient: a wave of it walks rows, two at a time."""
+    print("many rows", M, K, N, flush=True)
+    base.check_linear_backward("bf16", M, K, N, act="gelu", bias=True)
+    base.check_linear_backward("f16", M, K, N, bias=True)
+    base.check_gated_backward("f16", M, K, N, act="gelu", bias=True)

@@ -4,6 +4,7 @@ the allocation-free launch and a captured one ask for no more."""
 import ctypes
 import itertools
 import re
+import threading
 
 import pytest
 import torch
@@ -227,3 +228,44 @@ def test_a_launch_that_needs_no_workspace_is_captured_at_once(gpu):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shared", [False, True], ids=["two_streams", "one_stream"])
+def test_two_threads_launch_one_program(gpu, shared):
+    """Each thread its own sizes, of which one outgrows the other's workspace; on
+    streams of their own, or on one, where the launches take turns."""
+    g = gen_of("threads")
+    p = compiler.compile_program(operators.layer_norm_backward("bf16", residual=True))
+
+    def make(R, C):
+        x, dy, dres = (rand(g, (R, C), "bf16") for _ in range(3))
+        ins = [dy, x, rand(g, (C,), "bf16"), x.float().mean(1), x.float().std(1).reciprocal(), dres]
+        want = [empty((R, C), "bf16"), empty((C,), "bf16"), empty((C,), "bf16")]
+        compiler.compile_program(operators.layer_norm_backward("bf16", residual=True)).launch(ins + want)
+        return ins, want
+
+    work = [make(500, 300), make(700, 3000)]
+    runs = [[[torch.full_like(w, -1.0) for w in want] for _ in range(30)] for _, want in work]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    if shared:
+        streams[1] = streams[0]
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(i):
+        try:
+            for outs in runs[i]:
+                p.launch(work[i][0] + outs, stream=streams[i].cuda_stream)
+        except Exception as e:  # noqa: BLE001 (reported below)
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for (_, want), outs in zip(work, runs):
+        assert all(torch.equal(a, w) for o in outs for a, w in zip(o, want))
