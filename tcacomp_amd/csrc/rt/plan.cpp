@@ -554,11 +554,10 @@ bool WorkspaceLayout(const Plan& p, const std::vector<uint32_t>& dims, const std
     bool fits = true, records = false;
     for (int d : p.tensors[t].dims) fits = fits && times(&declared, dims[d]);
     for (const auto& k : p.kernels) {
-      if (k.scratch.empty() || !Selected(k, dims)) continue;
-      const uint64_t chunks = SplitChunks(k, dims);
       for (const auto& s : k.scratch) {
-        if (s.tensor != static_cast<int>(t)) continue;
+        if (s.tensor != static_cast<int>(t) || !Selected(k, dims)) continue;
         records = true;
+        const uint64_t chunks = SplitChunks(k, dims);
         if (k.split_dim >= 0 && chunks == 1) continue;
         size_t n = bytes;
         bool overflow = false;
