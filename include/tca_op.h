@@ -48,7 +48,9 @@
  * PAGE], row p % PAGE, its slot being page * PAGE + row. The new tokens of all
  * sequences are the rows of one batch of T, those of sequence s from starts[s]
  * to starts[s + 1] - 1. Lengths stay on the GPU: one captured launch serves every
- * batch of its extents.
+ * batch of its extents. Their lists (page_table's tensors, pos, slot, freq, table,
+ * starts, lens, lse) may start at any element, so that slices of longer lists do; all
+ * else starts on 16 bytes.
  *
  *   page_table            (no attributes; tensors i32)       free dim page, at least 1
  *       held [S], fresh [S], free [F], first [1]

@@ -15,6 +15,8 @@ may overlap). They are operators as those of ``operators`` are:
 
 A step of serving is these three launches whatever the lengths are, since those
 stay on the GPU: captured once, they replay for every batch of the same extents.
+The lists (the i32 tensors, freq and lse) may be slices of longer ones, of any
+start; x, y, q, k and v are 16-byte aligned at theirs.
 """
 from .operators import _listed, _make, Operator
 

@@ -137,6 +137,11 @@ class Writer {
     tensors_ << "tensor " << name << " " << elem << " " << role << " " << rank << " " << dims << "\n";
     types_[name] = std::make_pair(ElemType(elem), std::string(role) == "in");
   }
+  // A tensor of 4-byte values that kernels read and write one by one: it may start at any of them.
+  void List(const std::string& name, const std::string& elem, const char* role, const std::string& dims) {
+    Tensor(name, elem, role, dims);
+    tensors_ << "align " << name << " 4\n";
+  }
   bool Has(const std::string& tensor) const { return types_.count(tensor) != 0; }
   void Scalar(const std::string& name) {
     scalars_ << "scalar " << name << " f32\n";
@@ -717,16 +722,16 @@ void EmitPageTable(Writer* w) {
   w->Header("tca/hip/positions.h");
   for (const char* d : {"S", "S1", "F", "one", "P", "T"}) w->Dim(d, std::string(d) == "one" ? 1 : 0);
   w->Dim("page");
-  w->Tensor("held", "i32", "in", "S");
-  w->Tensor("fresh", "i32", "in", "S");
-  w->Tensor("free_pages", "i32", "in", "F");
-  w->Tensor("first", "i32", "in", "one");
-  w->Tensor("table", "i32", "out", "S P");
-  w->Tensor("starts", "i32", "out", "S1");
-  w->Tensor("lens", "i32", "out", "S");
-  w->Tensor("pos", "i32", "out", "T");
-  w->Tensor("slot", "i32", "out", "T");
-  w->Tensor("next", "i32", "out", "one");
+  w->List("held", "i32", "in", "S");
+  w->List("fresh", "i32", "in", "S");
+  w->List("free_pages", "i32", "in", "F");
+  w->List("first", "i32", "in", "one");
+  w->List("table", "i32", "out", "S P");
+  w->List("starts", "i32", "out", "S1");
+  w->List("lens", "i32", "out", "S");
+  w->List("pos", "i32", "out", "T");
+  w->List("slot", "i32", "out", "T");
+  w->List("next", "i32", "out", "one");
   w->Require("eq 1 S1/1 2 S/1 1/1");
   w->Require("le 1 1/1 1 page/1");
   Writer::Kernel k;
@@ -750,9 +755,9 @@ void EmitRotary(const Attrs& a, bool cache, Writer* w) {
   if (cache) {
     for (const char* d : {"T", "H", "D", "F", "HK", "G", "PAGES", "PAGE"}) w->Dim(d);
     w->Tensor("x", a.elem, "in", "T H D");
-    w->Tensor("pos", "i32", "in", "T");
-    w->Tensor("slot", "i32", "in", "T");
-    w->Tensor("freq", "f32", "in", "F");
+    w->List("pos", "i32", "in", "T");
+    w->List("slot", "i32", "in", "T");
+    w->List("freq", "f32", "in", "F");
     w->Tensor("q", a.elem, "out", "T HK G D");
     w->Tensor("k", a.elem, "out", "PAGES HK PAGE D");
     w->Tensor("v", a.elem, "out", "PAGES HK PAGE D");
@@ -760,8 +765,8 @@ void EmitRotary(const Attrs& a, bool cache, Writer* w) {
   } else {
     for (const char* d : {"T", "H", "D", "F"}) w->Dim(d);
     w->Tensor("x", a.elem, "in", "T H D");
-    w->Tensor("pos", "i32", "in", "T");
-    w->Tensor("freq", "f32", "in", "F");
+    w->List("pos", "i32", "in", "T");
+    w->List("freq", "f32", "in", "F");
     w->Tensor("y", a.elem, "out", "T H D");
   }
   w->Require("le 1 2*F/1 1 D/1");
@@ -805,11 +810,11 @@ void EmitPagedAttention(const Attrs& a, Writer* w) {
   w->Tensor("q", a.elem, "in", "T HK G D");
   w->Tensor("k", a.elem, "in", "PAGES HK PAGE D");
   w->Tensor("v", a.elem, "in", "PAGES HK PAGE D");
-  w->Tensor("table", "i32", "in", "S P");
-  w->Tensor("starts", "i32", "in", "S1");
-  w->Tensor("lens", "i32", "in", "S");
+  w->List("table", "i32", "in", "S P");
+  w->List("starts", "i32", "in", "S1");
+  w->List("lens", "i32", "in", "S");
   w->Tensor("y", a.elem, "out", "T HK G D");
-  if (stats) w->Tensor("lse", "f32", "out", "T HK G");
+  if (stats) w->List("lse", "f32", "out", "T HK G");
   w->Tensor("few_part", "f32", "local", "slots few_rows D");
   w->Tensor("few_ml", "f32", "local", "slots few_rows pair");
   w->Tensor("many_part", "f32", "local", "slots many_rows D");

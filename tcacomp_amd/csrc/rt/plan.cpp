@@ -178,6 +178,12 @@ bool Parse(const std::string& text, Plan* out, std::string* err) {
       }
       if (FindTensor(p, t.name) >= 0) return bad("duplicate tensor " + t.name);
       p.tensors.push_back(t);
+    } else if (kw == "align") {
+      uint64_t bytes = 0;
+      if (tok.size() != 3 || !ParseU64(tok[2], &bytes) || (bytes != 4 && bytes != 8 && bytes != 16)) return bad("align <tensor> <4|8|16>");
+      const int t = FindTensor(p, tok[1]);
+      if (t < 0 || p.tensors[t].role == Role::Local) return bad("align names no parameter " + tok[1]);
+      p.tensors[t].align = static_cast<uint32_t>(bytes);
     } else if (kw == "scalar") {
       if (tok.size() != 3) return bad("scalar <name> <dtype>");
       Scalar s{tok[1], DtypeFromName(tok[2])};
@@ -445,6 +451,8 @@ std::string Serialize(const Plan& p) {
     for (int d : t.dims) o << " " << p.dims[d].name;
     o << "\n";
   }
+  for (const auto& t : p.tensors)
+    if (t.align != 16u) o << "align " << t.name << " " << t.align << "\n";
   for (const auto& s : p.scalars) o << "scalar " << s.name << " " << DtypeName(s.dtype) << "\n";
   for (const auto& r : p.requires_) {
     o << "require " << kRequireNames[r.kind];
@@ -568,8 +576,8 @@ int Bind(const Plan& p, const tca_tensor* tensors, uint32_t n_tensors, const uin
       *err = "tensor " + t.name + " has a null data pointer";
       return TCA_ERR_INVALID;
     }
-    if (elems > 0 && (reinterpret_cast<uintptr_t>(a.data) % 16u) != 0u) {
-      *err = "tensor " + t.name + " data is not 16-byte aligned (vector loads need it)";
+    if (elems > 0 && (reinterpret_cast<uintptr_t>(a.data) % t.align) != 0u) {
+      *err = "tensor " + t.name + " data is not " + std::to_string(t.align) + "-byte aligned" + (t.align == 16u ? " (vector loads need it)" : "");
       return TCA_ERR_INVALID;
     }
     if (elems > kMaxElems) {

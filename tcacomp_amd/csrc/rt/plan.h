@@ -6,6 +6,8 @@
 //   program <name>
 //   dim <name> <extent>                        extent 0 = dynamic (u32 at run time)
 //   tensor <name> <dtype> <in|out|local> <rank> <dim-name>...
+//   align <tensor> <bytes>    where a parameter's data may start: on a multiple of 4, 8
+//       or 16 bytes (16 without the record; vectors of a tensor's rows need it)
 //   scalar <name> <dtype>
 //   require <eq|le|mod> <n> <term>... <n> <term>...    what the bound dims have to
 //       satisfy beyond the shape contract: the sum of the first terms equals the
@@ -89,6 +91,7 @@ struct Tensor {
   int dtype = TCA_F32;
   Role role = Role::In;
   std::vector<int> dims;  // indices into Plan::dims
+  uint32_t align = 16;    // bytes: where a parameter's data may start
 };
 
 struct Scalar {

@@ -120,7 +120,9 @@ struct tca_program_s {
   struct Prepared {
     uint32_t n_tensors = 0, n_free = 0;
     std::vector<uint32_t> key;        // per tensor: rank, dtype, dims...; then the free dims
-    std::vector<uint8_t> nonempty;    // per tensor parameter: it has elements (data must be valid)
+    // Per tensor parameter: the multiple its data has to start on, 0 where it has no
+    // elements (any pointer will do).
+    std::vector<uint32_t> align;
     std::vector<int> param_of;        // per plan tensor: its parameter index, -1 for a local
     std::vector<size_t> local_off;    // per plan tensor: offset of a local in the workspace
     // What the kernels use of the workspace at these dims, and what is allocated
@@ -491,6 +493,9 @@ int prepare_launch(tca_program p, const tca_tensor* tensors, uint32_t n_tensors,
   auto pr = std::make_shared<tca_program_s::Prepared>();
   pr->n_tensors = n_tensors;
   pr->n_free = n_free_dims;
+  std::vector<uint32_t> aligns;  // Bind has n_tensors parameters
+  for (const auto& t : pl.tensors)
+    if (t.role != tca::plan::Role::Local) aligns.push_back(t.align);
   for (uint32_t i = 0; i < n_tensors; ++i) {
     const tca_tensor& t = tensors[i];
     pr->key.push_back(t.rank);
@@ -500,7 +505,7 @@ int prepare_launch(tca_program p, const tca_tensor* tensors, uint32_t n_tensors,
       pr->key.push_back(t.dims[a]);
       elems *= t.dims[a];
     }
-    pr->nonempty.push_back(elems > 0 ? 1 : 0);
+    pr->align.push_back(elems > 0 ? aligns[i] : 0u);
   }
   for (uint32_t i = 0; i < n_free_dims; ++i) pr->key.push_back(free_dims[i]);
 
@@ -578,7 +583,7 @@ bool repeats(const tca_program_s::Prepared& pr, const tca_tensor* tensors, uint3
     if (t.rank != *k++ || static_cast<uint32_t>(t.dtype) != *k++) return false;
     for (uint32_t a = 0; a < t.rank; ++a)
       if (t.dims[a] != *k++) return false;
-    if (pr.nonempty[i] && (t.data == nullptr || (reinterpret_cast<uintptr_t>(t.data) % 16u) != 0u)) return false;
+    if (pr.align[i] != 0u && (t.data == nullptr || (reinterpret_cast<uintptr_t>(t.data) & (pr.align[i] - 1u)) != 0u)) return false;
   }
   for (uint32_t i = 0; i < n_free_dims; ++i)
     if (free_dims[i] != *k++) return false;
