@@ -150,7 +150,7 @@ def prepare(case, seed):
         col = torch.arange(table.shape[1], device=DEVICE)
         mine = col < _ints(have)[:, None]
         table[mine] = ids[:sum(have)]
-        free, t = ids[sum(have):].clone(), sum(fresh) + case["pad"]
+        free, t = ids[sum(have):].contiguous(), sum(fresh) + case["pad"]
         return {"case": case, "in": [_ints(held), _ints(fresh), free, _ints([1])],
                 "out": [table, empty(s + 1), empty(s), empty(t), empty(t), empty(1)]}
     e, d = case["elem"], case["d"]
