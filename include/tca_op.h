@@ -61,8 +61,9 @@
  *       are read. next: the first page not taken. starts, lens (held and new), pos
  *       and slot of each new token; rows behind the last token are -1. A token
  *       whose page lies behind the table's P columns or the list's end has slot -1
- *       (and such a column -1); tokens from T on are left out, and slots have to
- *       stay below 2^31.
+ *       (and such a column -1), and slots have to stay below 2^31. Tokens from T on
+ *       have no place in pos and slot (nothing stores their keys); table, starts,
+ *       lens and next are those of all new tokens whatever T is.
  *   rotary                elem=f32|bf16|f16 [interleaved] [inverse]       scalar scale
  *       x [T, H, D], pos [T] i32, freq [F] f32 -> y [T, H, D]             2 F <= D, F <= 512
  *       pair i < F of a head, (a, b) = x[i], x[F + i] (interleaved: x[2 i], x[2 i + 1]):

@@ -16,8 +16,9 @@ namespace hip {
 //
 // Every workgroup adds up all sequences (1024 runs of them, a scan in LDS) and
 // then places tokens, a grid's stride apart: one launch, no sums between
-// workgroups. A page's first token is always a new one, and stores its column:
-// nobody reads a column that this launch stores. Bound by the chain of loads, scan and
+// workgroups. A page's first token is always a new one, and stores its column, or, where
+// the batch has no room for that token, a lane of its own does: nobody reads a column
+// that this launch stores. Bound by the chain of loads, scan and
 // search: 256 sequences of one token 4.9 us, 37 prompts of 23 k tokens 6.1, 4096 sequences
 // of 107 k tokens 10.5 (18 with four tokens a lane).
 struct PageSeq {
@@ -32,6 +33,21 @@ __device__ __forceinline__ PageSeq page_seq(const int32_t* held, const int32_t* 
   const uint32_t need = ceil_div(q.held + q.fresh, page), most = need < P ? need : P;
   q.take = most > q.have ? most - q.have : 0u;
   return q;
+}
+// The page that column `col` of a sequence takes, `taken` pages after the first.
+__device__ __forceinline__ int32_t page_taken(const int32_t* free_pages, uint32_t F, int64_t from, uint64_t taken) {
+  const int64_t f = from + static_cast<int64_t>(taken);
+  return f >= 0 && f < static_cast<int64_t>(F) ? free_pages[f] : -1;
+}
+// Of 1024 runs whose sums end in ends[1 .. 1024], the one that holds unit t: ends[lo] <= t < ends[lo + 1].
+__device__ __forceinline__ uint32_t page_run(const uint64_t* ends, uint64_t t) {
+  uint32_t lo = 0u, hi = 1024u;
+  while (hi - lo > 1u) {
+    const uint32_t mid = (lo + hi) / 2u;
+    if (ends[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
 }
 __device__ __forceinline__ int32_t page_int(uint64_t v) { return v > 0x7fffffffu ? 0x7fffffff : static_cast<int32_t>(v); }
 
@@ -93,12 +109,7 @@ __device__ __forceinline__ void page_table(const int32_t* held, const int32_t* f
       pos[t] = slot[t] = -1;
       continue;
     }
-    uint32_t lo = 0u, hi = 1024u;  // tokens[lo] <= t < tokens[hi]
-    while (hi - lo > 1u) {
-      const uint32_t mid = (lo + hi) / 2u;
-      if (tokens[mid] <= t) lo = mid;
-      else hi = mid;
-    }
+    const uint32_t lo = page_run(tokens, t);
     uint64_t at = tokens[lo], taken = pages[lo];
     uint64_t s = static_cast<uint64_t>(lo) * run;
     PageSeq q = page_seq(held, fresh, s, page, P);
@@ -113,13 +124,27 @@ __device__ __forceinline__ void page_table(const int32_t* held, const int32_t* f
       if (col < q.have) {
         e = table[s * P + col];
       } else {
-        const int64_t f = from + static_cast<int64_t>(taken) + (col - q.have);
-        if (f >= 0 && f < static_cast<int64_t>(F)) e = free_pages[f];
+        e = page_taken(free_pages, F, from, taken + (col - q.have));
         if (in_page == 0u) table[s * P + col] = e;
       }
     }
     pos[t] = static_cast<int32_t>(p);
     slot[t] = e < 0 ? -1 : static_cast<int32_t>(static_cast<uint32_t>(e) * page + in_page);
+  }
+  if (tokens[1024] <= T) return;
+  // The columns whose first token is none of the batch's.
+  for (uint64_t k = blockIdx.x * 1024ull + tid; k < pages[1024]; k += gridDim.x * 1024ull) {
+    const uint32_t lo = page_run(pages, k);
+    uint64_t at = tokens[lo], taken = pages[lo];
+    uint64_t s = static_cast<uint64_t>(lo) * run;
+    PageSeq q = page_seq(held, fresh, s, page, P);
+    while (k >= taken + q.take && s + 1u < S) {  // ends: the run holds column k
+      at += q.fresh;
+      taken += q.take;
+      q = page_seq(held, fresh, ++s, page, P);
+    }
+    const uint32_t col = q.have + static_cast<uint32_t>(k - taken);
+    if (at + (static_cast<uint64_t>(col) * page - q.held) >= T) table[s * P + col] = page_taken(free_pages, F, from, k);
   }
 }
 

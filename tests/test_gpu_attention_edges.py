@@ -68,3 +68,30 @@ def test_lists_that_are_slices(gpu, by):
         want = launch_sliced(p, tensors, (), 0, **how)
         for got, w in zip(launch_sliced(p, tensors, set(which), by, **how), want):
             assert torch.equal(got.nan_to_num(3.0), w.nan_to_num(3.0)), p.name
+
+
+# ------------------------------------- batches shorter than the new tokens
+
+@pytest.mark.parametrize("S,new,page,columns,keep", [
+    (1, 40, 16, 4, 0.5), (1, 40, 16, 4, 0.0), (7, 40, 24, 5, 0.3), (64, 1, 16, 70, 0.6), (300, 9, 1, 30, 0.01), (1500, 30, 16, 4, 0.4), (3, 6000, 64, 100, 0.7)])
+def test_page_table_of_a_short_batch(gpu, S, new, page, columns, keep):
+    """Tokens from T on are in neither pos nor slot; the table's columns, starts, lens
+    and the next free page are those of all new tokens."""
+    print("short table", S, new, page, keep, flush=True)
+    rng = random.Random(S * 100 + page)
+    fresh = [rng.choice((0, 1, new, rng.randint(0, new))) for _ in range(S)]
+    fresh[S // 2] = new
+    held = [rng.randint(0, columns * page - 1) for _ in range(S)]
+    ids = list(range(S * columns + 9))
+    rng.shuffle(ids)
+    table, at = [], 0
+    for h in held:
+        n = -(-h // page)
+        table.append(ids[at:at + n] + [-5] * (columns - n))
+        at += n
+    free = ids[at:at + max(1, sum(-(-n // page) for n in fresh) - 1)]
+    T = int(sum(fresh) * keep)
+    got = launch_page_table(held, fresh, free, 1, table, page, T)
+    want = ref.page_table(held, fresh, free, 1, table, page, sum(fresh))
+    for g, w, what in zip(got, want, ("table", "starts", "lens", "pos", "slot", "next")):
+        assert g == ([w] if what == "next" else w[:T] if what in ("pos", "slot") else w), what
