@@ -83,7 +83,8 @@
  *       whose entry of the table names no page or lies behind its P columns.
  *       y = sum_j p_j v_j, p the softmax of scale q . k_j; lse = log sum_j exp(scale q . k_j),
  *       to merge with attention over other keys. A row that sees no key has y = 0
- *       and lse = -inf. Rows that no sequence has are left as they were; starts
+ *       and lse = -inf. Rows that no sequence has are left as they were; of starts that
+ *       go past T, the rows that are there keep their positions; starts
  *       have to ascend (rows that two sequences name are stored by either). Scores
  *       and sums are 32-bit; probabilities are rounded to elem for the product
  *       with v. Values that are not finite reach the rows that see them only. Up to

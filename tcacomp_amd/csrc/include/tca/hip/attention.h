@@ -70,7 +70,7 @@ struct AttendShape {
 
 // One sequence: its rows in the batch and its place in the cache.
 struct AttendSeq {
-  uint32_t start, n, limit;  // first row, new tokens, keys that the table can name
+  uint32_t start, n, limit;  // first row, rows in the batch, keys that the table can name
   int32_t base;              // the first new token's position
 };
 __device__ __forceinline__ AttendSeq attend_seq(const AttendShape& a, uint32_t s) {
@@ -83,7 +83,9 @@ __device__ __forceinline__ AttendSeq attend_seq(const AttendShape& a, uint32_t s
   const uint32_t L = len < 0 ? 0u : static_cast<uint32_t>(len);
   const uint64_t room = a.PAGES == 0u ? 0u : static_cast<uint64_t>(a.P) * a.PAGE;
   q.limit = L < room ? L : static_cast<uint32_t>(room);
-  q.base = static_cast<int32_t>(L) - static_cast<int32_t>(q.n);
+  // Rows behind the batch are none of it but count for the others' positions. (Those
+  // before row 0 do not: positions are counted from the last row.)
+  q.base = q.n == 0u ? 0 : static_cast<int32_t>(L) - (e - static_cast<int32_t>(q.start));
   return q;
 }
 

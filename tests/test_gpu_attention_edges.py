@@ -95,3 +95,126 @@ def test_page_table_of_a_short_batch(gpu, S, new, page, columns, keep):
     want = ref.page_table(held, fresh, free, 1, table, page, sum(fresh))
     for g, w, what in zip(got, want, ("table", "starts", "lens", "pos", "slot", "next")):
         assert g == ([w] if what == "next" else w[:T] if what in ("pos", "slot") else w), what
+
+
+def whole(elem, case, scale, window=0):
+    """attention_ref.paged_attention of a case whose starts go past its rows: of a batch
+    that has them all, cut to the rows that are there."""
+    q, k, v, table, starts, lens = case
+    T = q.shape[0]
+    rest = torch.zeros((max(starts[-1] - T, 0),) + q.shape[1:], device=q.device, dtype=q.dtype)
+    return [t[:T] for t in ref.paged_attention(torch.cat([q, rest]), k, v, table, starts, lens, scale, window, DTYPES[elem])]
+
+
+def agree(y, lse, want, rows=slice(None)):
+    """Values within their bounds; NaN (of rows that see it) and -inf in the same places."""
+    y, lse, (wy, wl, by, bl) = y[rows], lse[rows], (t[rows] for t in want)
+    none = wl == -float("inf")
+    assert torch.equal(none, lse == -float("inf")) and torch.equal(wy.isnan(), y.isnan()) and torch.equal(wl.isnan(), lse.isnan())
+    odd, wild = wy.isnan(), none | wl.isnan()
+    close(torch.where(odd, 0.0, y), torch.where(odd, 0.0, wy), torch.where(odd, 1.0, by), "y")
+    close(torch.where(wild, 0.0, lse), torch.where(wild, 0.0, wl), torch.where(wild, 1.0, bl), "lse")
+
+
+@pytest.mark.parametrize("elem", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,fresh,G,D,T,window", [
+    ([100], [10], 4, 64, 3, 0), ([700, 90], [300, 30], 4, 64, 310, 0), ([700, 90], [300, 30], 2, 128, 170, 0), ([50, 50, 50], [20, 20, 20], 1, 256, 25, 0),
+    ([3000, 40], [6, 8], 4, 128, 9, 0), ([900, 800], [400, 300], 2, 64, 500, 33)])
+def test_attention_of_a_short_batch(gpu, elem, lens, fresh, G, D, T, window):
+    """Rows keep the positions that starts and lens give them, whether the batch has the rows behind them or not."""
+    print("short batch", lens, fresh, T, flush=True)
+    q, k, v, table, starts, lens = make(gen_of("cut", T, D, elem), elem, lens, fresh, 2, G, D, 16)
+    case = (q[:T].contiguous(), k, v, table, starts, lens)
+    y, lse = run(elem, case, D ** -0.5, window)
+    agree(y, lse, whole(elem, case, D ** -0.5, window))
+
+
+def test_a_step_of_a_short_batch(gpu):
+    """Tables, stores and attention of a batch with room for some of the new tokens
+    only: its rows are those of a batch with room for all, no page is lost, and a
+    sequence that was there as a whole goes on."""
+    S, HK, G, D, page, columns = 3, 2, 4, 64, 16, 8
+    g = gen_of("short step")
+    freq = torch.rand(D // 2, generator=g, device="cuda")
+    fresh, T = [30, 50, 21], 62  # all of the first sequence, some of the second, none of the third
+    x = rand(g, (sum(fresh), HK * (G + 2), D), "bf16")
+    free = torch.randperm(S * columns, generator=g, device="cuda").int()
+
+    class State:
+        def __init__(self):
+            self.table = torch.full((S, columns), -1, device="cuda", dtype=torch.int32)
+            self.k, self.v = (torch.full((S * columns, HK, page, D), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+            self.held, self.first = ints([0] * S), ints([0])
+
+        def step(self, new, x):
+            T = x.shape[0]
+            starts, lens, pos, slot, after = ints([0] * (S + 1)), ints([0] * S), ints([0] * T), ints([0] * T), ints([0])
+            q = torch.zeros((T, HK, G, D), device="cuda", dtype=x.dtype)
+            y, lse = torch.full_like(q, -12345.0), torch.zeros((T, HK, G), device="cuda")
+            program(attention.page_table).launch([self.held, ints(new), free, self.first, self.table, starts, lens, pos, slot, after], free_dims=(page,))
+            program(attention.rotary_cache, "bf16").launch([x, pos, slot, freq, q, self.k, self.v], scalars=(1.0,))
+            program(attention.paged_attention, "bf16", False, True).launch([q, self.k, self.v, self.table, starts, lens, y, lse], scalars=(D ** -0.5,))
+            want = whole("bf16", (q, self.k, self.v, self.table, starts.tolist(), lens.tolist()), D ** -0.5)
+            self.held, self.first = lens, after
+            return q, y, lse, want
+
+    full, short = State(), State()
+    q, _, _, want = full.step(fresh, x)
+    q2, y, lse, _ = short.step(fresh, x[:T].contiguous())
+    assert torch.equal(q2, q[:T])
+    for name in ("table", "held", "first"):
+        assert torch.equal(getattr(short, name), getattr(full, name)), name
+    agree(y, lse, [w[:T] for w in want])
+    more = rand(g, (5, HK * (G + 2), D), "bf16")
+    _, _, _, want = full.step([5, 0, 0], more)
+    _, y, lse, _ = short.step([5, 0, 0], more)
+    agree(y, lse, want)
+
+
+def test_starts_and_lengths_that_leave_the_batch(gpu):
+    """Against the rows that are there, between guards that nothing writes; of a cache
+    whose rows past the sequences hold NaN, and of one that is finite."""
+    q, k, v, table, _, _ = make(gen_of("leave"), "bf16", [100, 100, 100], [1, 1, 1], 2, 4, 64, 16)
+    for k, v in ((k, v), (k.nan_to_num(0.5), v.nan_to_num(-0.25))):
+        leave_the_batch(q, k, v, table)
+
+
+def leave_the_batch(q, k, v, table):
+    T, guard = 3, 2
+    cases = [  # starts, lens; the same with starts inside, as the reference takes them: (starts, lens, rows to check)
+        ([0, 2, 1, 900], [100, -5, 100], None, [0]),
+        ([-3, 2, 2, 2], [100, 100, 100], ([0, 2, 2, 2], [100, 100, 100]), [0, 1]),
+        ([-(1 << 31), 2, 2, 3], [100, 100, 77], ([0, 2, 2, 3], [100, 100, 77]), [0, 1, 2]),
+        ([0, 2, 2, 3], [1 << 20, 5, (1 << 31) - 1], ([0, 2, 2, 3], [1 << 20, 5, (1 << 31) - 1]), [0, 1, 2]),
+        ([0, 1, 3, 3], [1, -(1 << 31), 8], ([0, 1, 3, 3], [1, 0, 8]), [0, 1, 2]),
+        ([2, 1, 0, 0], [100, 100, 100], ([0, 0, 0, 0], [0, 0, 0]), []),
+        ([3, (1 << 31) - 1, 5, 9], [100, 100, 100], ([0, 0, 0, 0], [0, 0, 0]), []),
+        ([0, 1, 1, 900], [100, -5, 1000], ([0, 1, 1, 900], [100, 0, 1000]), [0, 1, 2]),
+    ]
+    for starts, lens, inside, rows in cases:
+        print(starts, lens, flush=True)
+        y = torch.full((T + 2 * guard,) + q.shape[1:], -12345.0, device="cuda", dtype=q.dtype)
+        lse = torch.full((T + 2 * guard,) + q.shape[1:3], -12345.0, device="cuda")
+        program(attention.paged_attention, "bf16", False, True).launch(
+            [q, k, v, table, ints(starts), ints(lens), y[guard:guard + T], lse[guard:guard + T]], scalars=(0.125,))
+        for t in (y, lse):
+            assert (t[:guard] == -12345.0).all() and (t[guard + T:] == -12345.0).all()
+        y, lse = y[guard:guard + T], lse[guard:guard + T]
+        if inside is None:  # row 1 is either sequence's; row 2 lies 798 before the third sequence's first key
+            want = ref.paged_attention(q, k, v, table, [0, 2, 2, 2], [100, 0, 0], 0.125, 0, DTYPES["bf16"])
+            assert (y[2] == 0).all() and (lse[2] == -float("inf")).all()
+            assert ((y[1] == 0).all() and (lse[1] == -float("inf")).all()) or ((y[1].double() - want[0][1]).abs() <= want[2][1]).all()
+        else:
+            want = whole("bf16", (q, k, v, table, *inside), 0.125)
+        agree(y, lse, want, rows)
+        left = [r for r in range(T) if r not in rows] if inside is not None else []
+        assert (y[left] == -12345.0).all() and (lse[left] == -12345.0).all()
+
+
+def test_no_sequences_and_no_columns(gpu):
+    """No sequence at all leaves every row; a table without columns hides every key."""
+    q, k, v, table, starts, lens = make(gen_of("none"), "bf16", [40, 90], [3, 40], 2, 4, 64, 16)
+    y, lse = run("bf16", (q, k, v, table[:0], [0], []), 0.125)
+    assert (y == -12345.0).all() and (lse == -12345.0).all()
+    y, lse = run("bf16", (q, k, v, table[:, :0].contiguous(), starts, lens), 0.125)
+    assert (y == 0).all() and (lse == -float("inf")).all()
