@@ -84,12 +84,12 @@
  *       y = sum_j p_j v_j, p the softmax of scale q . k_j; lse = log sum_j exp(scale q . k_j),
  *       to merge with attention over other keys. A row that sees no key has y = 0
  *       and lse = -inf. Rows that no sequence has are left as they were; of starts that
- *       go past T, the rows that are there keep their positions; starts
- *       have to ascend (rows that two sequences name are stored by either). Scores
- *       and sums are 32-bit; probabilities are rounded to elem for the product
- *       with v. Values that are not finite reach the rows that see them only. Up to
- *       67 MB of workspace, and more than the allocation-free launch has where T G
- *       is above 94 rows of 128 features.
+ *       go past T, the rows that are there keep their positions; starts have to
+ *       ascend (rows that two sequences name are stored by either). Scores and sums
+ *       are 32-bit; probabilities are rounded to elem for the product with v. Values
+ *       that are not finite reach the rows that see them only. 77 MB of workspace at
+ *       128 features, up to 85; the allocation-free launch has enough for T G of at
+ *       most 93 rows of 128 features.
  *
  * y may be x in rotary; otherwise nothing of theirs overlaps.
  */

@@ -804,6 +804,7 @@ void EmitPagedAttention(const Attrs& a, Writer* w) {
   w->Dim("slots", 512);
   w->Dim("few_rows", 32);
   w->Dim("many_rows", 256);
+  w->Dim("wide_rows", 128);  // of tiles of heads above 128
   w->Dim("pair", 2);
   w->Dim("groups", 256);
   w->Dim("words", 8);
@@ -819,6 +820,8 @@ void EmitPagedAttention(const Attrs& a, Writer* w) {
   w->Tensor("few_ml", "f32", "local", "slots few_rows pair");
   w->Tensor("many_part", "f32", "local", "slots many_rows D");
   w->Tensor("many_ml", "f32", "local", "slots many_rows pair");
+  w->Tensor("wide_part", "f32", "local", "slots wide_rows D");
+  w->Tensor("wide_ml", "f32", "local", "slots wide_rows pair");
   w->Tensor("few_join", "u32", "local", "groups words");
   w->Tensor("many_join", "u32", "local", "groups words");
   w->Scalar("scale");
@@ -832,27 +835,29 @@ void EmitPagedAttention(const Attrs& a, Writer* w) {
   for (uint32_t dp : {64u, 128u, 192u, 256u}) {
     const std::string DP = std::to_string(dp);
     const uint32_t rows = dp <= 128u ? 256u : 128u;
+    const std::string big = dp <= 128u ? "many" : "wide";  // whose locals: a launch allocates those that its kernels take
     const std::string head = "  const tca::hip::AttendShape a = {table, starts, lens, T, HK, G, D, PAGES, PAGE, S, P, " +
                              std::string(window ? "window" : "0u") + "};\n";
-    auto out = [&](const char* name, uint32_t most) {
-      const std::string n = std::string(name) + "_";
-      return std::string("  const tca::hip::AttendOut<") + T + "> " + name + " = {y, " + (stats ? "lse" : "(float*)nullptr") + ", " + n +
-             "part, reinterpret_cast<float2*>(" + n + "ml), " + n + "join, tca::hip::attend_part_rows(T, G, " + std::to_string(most) + "u)};\n";
+    auto out = [&](const std::string& name, const std::string& parts, uint32_t most) {
+      return std::string("  const tca::hip::AttendOut<") + T + "> " + name + " = {y, " + (stats ? "lse" : "(float*)nullptr") + ", " + parts +
+             "_part, reinterpret_cast<float2*>(" + parts + "_ml), " + name + "_join, tca::hip::attend_part_rows(T, G, " + std::to_string(most) +
+             "u)};\n";
     };
+    const std::string outs = out("few", "few", 32) + out("many", big, rows);
     auto records = [&]() {
       std::vector<std::string> r = {When("D", from, dp)};
-      for (const char* n : {"few", "many"}) {
-        const std::string most = std::to_string(n[0] == 'f' ? 32u : rows);
-        r.push_back(Scratch(std::string(n) + "_part", "512/1 T*G/1:" + most + " D/1"));
-        r.push_back(Scratch(std::string(n) + "_ml", "1024/1 T*G/1:" + most));
+      for (const std::string& n : {std::string("few"), big}) {
+        const std::string most = std::to_string(n == "few" ? 32u : rows);
+        r.push_back(Scratch(n + "_part", "512/1 T*G/1:" + most + " D/1"));
+        r.push_back(Scratch(n + "_ml", "1024/1 T*G/1:" + most));
       }
       return r;
     };
-    const std::string outs = std::string("y ") + (stats ? "lse " : "") + "few_part few_ml many_part many_ml few_join many_join T HK G D";
+    const std::string written = std::string("y ") + (stats ? "lse " : "") + "few_part few_ml " + big + "_part " + big + "_ml few_join many_join T HK G D";
     Writer::Kernel k;
     k.suffix = "_" + DP;
-    k.params = "q k v table starts lens " + outs + " PAGES PAGE S P" + (window ? " window" : "") + " scale";
-    k.body = head + out("few", 32) + out("many", rows) + "  tca::hip::attend<" + f16 + ", " + DP +
+    k.params = "q k v table starts lens " + written + " PAGES PAGE S P" + (window ? " window" : "") + " scale";
+    k.body = head + outs + "  tca::hip::attend<" + f16 + ", " + DP +
              ">(a, q, k, v, reinterpret_cast<const uint4*>(tca::hip::kAttendZero), few, many, scale);\n";
     k.grid = "256/1 T*HK/1:1 G/1:1";
     k.block = dp <= 128u ? 512 : 256;
@@ -863,7 +868,7 @@ void EmitPagedAttention(const Attrs& a, Writer* w) {
     Writer::Kernel j;
     j.suffix = "_" + DP + "join";
     j.params = k.params;
-    j.body = head + out("few", 32) + out("many", rows) + "  tca::hip::join_attention<" + f16 + ", " + DP + ">(a, q, k, v, few, many, scale);\n";
+    j.body = head + outs + "  tca::hip::join_attention<" + f16 + ", " + DP + ">(a, q, k, v, few, many, scale);\n";
     // Workgroups of a tile: one for each 256 of its four-column pieces, at most 8 (prompts of
     // 4096: 57 us with one, 17 with 8).
     j.grid = "256/1 T*G*D/1024:8 HK/1:1";

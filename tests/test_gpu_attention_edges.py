@@ -218,3 +218,18 @@ def test_no_sequences_and_no_columns(gpu):
     assert (y == -12345.0).all() and (lse == -12345.0).all()
     y, lse = run("bf16", (q, k, v, table[:, :0].contiguous(), starts, lens), 0.125)
     assert (y == 0).all() and (lse == -float("inf")).all()
+
+
+def test_the_largest_batch_of_the_allocation_free_launch(gpu):
+    """512 (min(T, 32) + T) (4 D + 8) bytes and 16 KiB of its 32 MiB."""
+    from tcacomp_amd import _lib
+    for T, D, fits in ((93, 128, True), (94, 128, False), (31, 256, True), (32, 256, False)):
+        case = make(gen_of("fits", T, D), "bf16", [2000], [T], 2, 1, D, 16)
+        y, lse = run("bf16", case, D ** -0.5)
+        agree(y, lse, whole("bf16", case, D ** -0.5))
+        if fits:
+            y2, lse2 = run("bf16", case, D ** -0.5, noalloc=True)
+            assert torch.equal(y, y2) and torch.equal(lse, lse2)
+        else:
+            with pytest.raises(_lib.TcaError, match="scratch"):
+                run("bf16", case, D ** -0.5, noalloc=True)
