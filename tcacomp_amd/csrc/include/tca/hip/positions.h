@@ -307,7 +307,7 @@ __device__ __forceinline__ void rotary_cache(const T* x, const int32_t* pos, con
       continue;
     }
     const int32_t at = slot[t0 + n];
-    if (at < 0) continue;
+    if (at < 0 || PAGE == 0u) continue;  // pages of no tokens have no slot
     const uint32_t p = static_cast<uint32_t>(at) / PAGE, o = static_cast<uint32_t>(at) - p * PAGE;
     if (p >= PAGES) continue;
     const bool value = h >= HK * (G + 1u);

@@ -233,3 +233,21 @@ def test_the_largest_batch_of_the_allocation_free_launch(gpu):
         else:
             with pytest.raises(_lib.TcaError, match="scratch"):
                 run("bf16", case, D ** -0.5, noalloc=True)
+
+
+def test_pages_of_no_tokens(gpu):
+    """A cache [9, 2, 0, 64]: no slot lies in it, no key is seen; queries are turned as ever."""
+    g = gen_of("page 0")
+    x, pos, freq = rand(g, (5, 8, 64), "bf16"), ints([3, 1, 4, 1, 5]), torch.rand(32, generator=g, device="cuda")
+    outs = []
+    for page, slot in ((0, [0, 1, 7, 1 << 30, 8]), (16, [-1] * 5)):
+        q = torch.zeros((5, 2, 2, 64), device="cuda", dtype=torch.bfloat16)
+        k, v = (rand(g, (9, 2, page, 64), "bf16") for _ in range(2))
+        program(attention.rotary_cache, "bf16").launch([x, pos, ints(slot), freq, q, k, v], scalars=(1.0,))
+        outs.append(q)
+    assert torch.equal(outs[0], outs[1]) and outs[0].any()
+    k = torch.zeros((9, 2, 0, 64), device="cuda", dtype=torch.bfloat16)
+    for starts in ([0, 5], [0, 1]):
+        y, lse = run("bf16", (outs[0], k, k.clone(), ints([[0, 1, 2]]), starts, [40]), 0.125)
+        n = starts[1]
+        assert (y[:n] == 0).all() and (lse[:n] == -float("inf")).all() and (y[n:] == -12345.0).all() and (lse[n:] == -12345.0).all()
