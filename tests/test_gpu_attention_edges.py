@@ -251,3 +251,72 @@ def test_pages_of_no_tokens(gpu):
         y, lse = run("bf16", (outs[0], k, k.clone(), ints([[0, 1, 2]]), starts, [40]), 0.125)
         n = starts[1]
         assert (y[:n] == 0).all() and (lse[:n] == -float("inf")).all() and (y[n:] == -12345.0).all() and (lse[n:] == -12345.0).all()
+
+
+# ------------------- values that are not finite, anywhere in a workgroup's run
+
+def units(lens, fresh, HK, G, D, window=0):
+    """(many, few): units of work of each kind, as the kernels count them."""
+    most, many, few = (256, 0, 0) if D <= 128 else (128, 0, 0)
+    keys_few = 256 if D <= 128 else 128
+    heads = min(G, most)
+    for L, n in zip(lens, fresh):
+        if n == 0:
+            continue
+        big = n * G > 32
+        step, block = (most // heads, 64) if big else (n, keys_few)
+        total = 0
+        for t0 in range(0, n, step):
+            hi, lo = L - n + min(n, t0 + step), max(0, L - n + t0 + 1 - window) if window else 0
+            total += max(1, (hi - 1) // block + 1 - lo // block if hi > lo else 0)
+        total *= HK * (-(-G // heads) if big else 1)
+        many, few = (many + total, few) if big else (many, few + total)
+    return many, few
+
+
+SHORT = [33 + 7 * i % 30 for i in range(150)]  # tiles of one block each
+ODD = {  # lengths, new tokens, key heads, group, features, window, (sequence, place among its new tokens), units of a workgroup at least (many, few)
+    "prompt": ([2500], [2500], 2, 1, 64, 0, [(0, 1203)], (2, 0)),
+    "prompt f": ([1700, 33], [1700, 33], 2, 4, 128, 0, [(0, 700)], (3, 0)),
+    "wide": ([1500, 300], [1500, 200], 2, 2, 256, 0, [(0, 800), (1, 3)], (3, 0)),
+    "window": ([4000], [3000], 2, 2, 64, 300, [(0, 1501)], (2, 0)),
+    "short ones": (SHORT, SHORT, 6, 1, 64, 0, [(76, 20)], (4, 0)),
+    "short beside long": ([2100] + SHORT, [2100] + SHORT, 3, 2, 64, 0, [(0, 1000), (41, 17), (149, 30)], (6, 0)),
+    "few": ([9000, 5000], [4, 7], 8, 4, 128, 0, [(0, 2), (1, 3)], (0, 2)),
+    "few f": ([9001], [6], 2, 5, 64, 0, [(0, 3)], (0, 1)),
+    "few wide": ([7000, 3000, 50], [3, 1, 8], 4, 4, 192, 0, [(0, 1), (2, 4)], (0, 1)),
+    "few window": ([9000, 4000], [4, 8], 8, 4, 64, 3500, [(0, 1)], (0, 1)),
+    "both": ([5000, 1900, 3000, 60], [5, 1000, 1, 60], 4, 4, 128, 0, [(0, 2), (1, 500)], (4, 1)),
+}
+
+
+@pytest.mark.parametrize("name", sorted(ODD))
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+def test_values_that_are_not_finite_in_any_tile(gpu, name, bad):
+    """A value of one key head of a new token: rows before it, rows whose window has left
+    it, other heads and other sequences are as without it."""
+    lens, fresh, HK, G, D, window, where, (many, few) = ODD[name]
+    elem = "f16" if name.endswith("f") else "bf16"
+    print(name, bad, elem, flush=True)
+    counted = units(lens, fresh, HK, G, D, window)
+    assert -(-counted[0] // 256) >= many and -(-counted[1] // 256) >= few, counted
+    case = make(gen_of("any tile", name), elem, lens, fresh, HK, G, D, 16, pad=1)
+    q, k, v, table, starts, _ = case
+    want = ref.paged_attention(*case, D ** -0.5, window, DTYPES[elem])  # without them
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    for s, i in where:
+        at, h = lens[s] - fresh[s] + i, (s + i) % HK
+        v[int(table[s, at // 16]), h, at % 16, D // 2] = float(bad)
+        last = fresh[s] if not window else min(fresh[s], i + window)
+        hit[starts[s] + i:starts[s] + last, h] = True
+    y, lse = run(elem, case, D ** -0.5, window)
+    n = starts[-1]
+    assert (y[n:] == -12345.0).all() and (lse[n:] == -12345.0).all()
+    free = ~hit[:n]
+    close(y[:n][free], want[0][:n][free], want[2][:n][free], "rows that do not see it")
+    close(lse[:n], want[1][:n], want[3][:n], "the statistics, which no value enters")
+    column = y[:n, :, :, D // 2][hit[:n]]
+    assert column.isnan().all() if bad == "nan" else (column == float("inf")).all()
+    rest = torch.ones(D, dtype=torch.bool, device="cuda")
+    rest[D // 2] = False
+    close(y[:n][hit[:n]][..., rest], want[0][:n][hit[:n]][..., rest], want[2][:n][hit[:n]][..., rest], "other columns of rows that see it")
