@@ -868,6 +868,7 @@ void EmitPagedAttention(const Attrs& a, Writer* w) {
     Writer::Kernel j;
     j.suffix = "_" + DP + "join";
     j.params = k.params;
+    j.waves = 6;  // the join's loads in flight: what follows a flagged tile would take more registers
     j.body = head + outs + "  tca::hip::join_attention<" + f16 + ", " + DP + ">(a, q, k, v, few, many, scale);\n";
     // Workgroups of a tile: one for each 256 of its four-column pieces, at most 8 (prompts of
     // 4096: 57 us with one, 17 with 8).

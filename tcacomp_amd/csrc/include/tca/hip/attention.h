@@ -19,7 +19,8 @@
 // 6 us behind a chain of lengths, table, keys; 64 sequences of half as many keys: 273 and
 // 5, 5.8 TB/s. Four chunks of 512 over 8000 to 16000 keys, 8 heads of a group: 400 us and
 // 14, 1.0 PFLOP/s (the matrix cores busy for 49% of the cycles); prompts of 4096 (f16) 385
-// and 14, 0.71. Everything runs once; a row of values that are not finite twice.
+// and 14, 0.71. Everything runs once, but rows of a tile that a value which is not finite
+// has got into though they do not see it: without the matrix cores (redo_rows).
 //
 // Lengths lie on the GPU, so the launch knows shapes only: every workgroup of
 // a fixed grid reads the lengths, counts the work of all sequences in units
@@ -599,8 +600,8 @@ struct AttendV {
 
 // Whether sums of a row are not finite. A row that does not see a key has
 // probability 0 for it, and the product of 0 and a value that is not finite is NaN:
-// where rows of different positions share a block, such rows are done again by
-// themselves (redo_rows), from a flag of the workgroup.
+// where rows of different positions share a block, a flag of the workgroup has those
+// that this has happened to done again (redo_rows).
 template <uint32_t DP>
 __device__ __forceinline__ bool attend_odd(const AttendAcc<DP, 1>& acc) {
   float z = 0.0f;
@@ -1212,57 +1213,151 @@ __device__ __forceinline__ void join_kind(const AttendShape& a, const AttendOut<
     attend_store<F16>(a, t, out, -1, r, d, s.o, s.m, s.l);
   }
 }
-// One row by a wave, its keys alone: 64 scores at a time, a lane each, then their
-// values, four columns a lane.
+// Which columns of the keys that some of a tile's rows see and others do not hold values
+// that are not finite: the least such key and the one after the greatest, of all of them
+// ([0], [1]) and of NaN alone.
+struct AttendOdd {
+  uint32_t bad[2][256], nan[2][256], rows[512];
+};
+// Whether what row's keys [lo, hi) give column d can be off: a key that it does not see
+// holds such a value there, and none that it sees is known to be NaN (as its own key's is
+// where a whole sequence is).
+__device__ __forceinline__ bool attend_off(const AttendOdd& odd, uint32_t d, uint32_t lo, uint32_t hi) {
+  if (odd.bad[0][d] >= lo && odd.bad[1][d] <= hi) return false;
+  const uint32_t first = odd.nan[0][d], last = odd.nan[1][d];
+  return !((first >= lo && first < hi) || (last > lo && last <= hi));
+}
+template <typename T>
+__device__ __forceinline__ void attend_find_odd(const AttendShape& a, const AttendTile& t, const T* v, AttendOdd* odd) {
+  const uint32_t tid = threadIdx.x, D4 = a.D / 4u;
+  const uint32_t lo = attend_begin(a, t.q, t.t0), hi = attend_end(t.q, t.t1);
+  // Every row sees the keys from `from` to `to` (the first row's own, which is looked at
+  // all the same); there are less than 256 on either side.
+  const uint32_t from = attend_begin(a, t.q, t.t1 - 1u), to = attend_end(t.q, t.t0 + 1u);
+  const uint32_t back = to > lo ? to - 1u : lo;
+  __syncthreads();  // the last tile's have been read
+  odd->bad[0][tid] = odd->nan[0][tid] = 0xffffffffu;
+  odd->bad[1][tid] = odd->nan[1][tid] = 0u;
+  const uint32_t low = from < hi ? from : hi, before = low > lo ? low - lo : 0u, after = hi > back ? hi - back : 0u;
+  for (uint32_t i = tid; i < before + after; i += 256u)
+    odd->rows[i] = attend_key(a, t, i < before ? lo + i : back + (i - before), lo, hi);
+  __syncthreads();
+  for (uint32_t i = tid; i < (before + after) * D4; i += 256u) {
+    const uint32_t n = i / D4, d = (i - n * D4) * 4u, off = odd->rows[n], key = n < before ? lo + n : back + (n - before);
+    if (off == kNoRow) continue;
+    const vec<T, 4> x = load_vec<T, 4>(v + static_cast<uint64_t>(off) * 8u + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float f = static_cast<float>(x[e]);
+      if (f - f == 0.0f) continue;
+      atomicMin(&odd->bad[0][d + e], key);
+      atomicMax(&odd->bad[1][d + e], key + 1u);
+      if (f == f) continue;
+      atomicMin(&odd->nan[0][d + e], key);
+      atomicMax(&odd->nan[1][d + e], key + 1u);
+    }
+  }
+  __syncthreads();
+}
+// Of kRedo rows from r0 on, those of `which` by a wave over all that they see: 64 scores
+// at a time, a lane each, then their values, four columns a lane. Bound by the latency of
+// the loads: 30 us for 64 keys, by 32 waves a tile. (What stands here takes registers from
+// the join of every launch: four rows at a time are 1.2 times as fast, in 88 to 98
+// registers, with which the join of 64 single tokens takes 6.9 us for 6.1.)
+constexpr uint32_t kRedo = 2;
 template <bool F16, typename T>
-__device__ __forceinline__ void redo_row(const AttendShape& a, const AttendTile& t, uint32_t r, const AttendOut<T>& out, const T* q, const T* k,
-                                         const T* v, float scale2, uint32_t lane) {
-  const uint32_t row = attend_row(a, t, r);
-  if (row == kNoRow) return;
-  const uint32_t token = t.t0 + r / t.stride, lo = attend_begin(a, t.q, token), hi = attend_end(t.q, token + 1u), D8 = a.D / 8u;
-  const uint4* q8 = reinterpret_cast<const uint4*>(q) + static_cast<uint64_t>(row) * D8;
-  float m = -__builtin_inff(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t j0 = lo; j0 < hi; j0 += 64u) {
-    const uint32_t off = attend_key(a, t, j0 + lane, lo, hi);
-    float s = 0.0f;
-    for (uint32_t c = 0u; off != kNoRow && c < D8; ++c) {
-      const vec<T, 8> x = __builtin_bit_cast(vec<T, 8>, q8[c]), y = __builtin_bit_cast(vec<T, 8>, reinterpret_cast<const uint4*>(k)[static_cast<uint64_t>(off) + c]);
+__device__ __forceinline__ void redo_some(const AttendShape& a, const AttendTile& t, uint32_t r0, uint32_t which, const AttendOut<T>& out, const T* q,
+                                          const T* k, const T* v, float scale2, uint32_t lane) {
+  const uint32_t D8 = a.D / 8u, any = r0 + static_cast<uint32_t>(__builtin_ctz(which));
+  uint32_t row[kRedo], lo[kRedo], hi[kRedo], least = 0xffffffffu, most = 0u;
+  float m[kRedo], l[kRedo], o[kRedo][4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf(static_cast<float>(x[e]), static_cast<float>(y[e]), s);
+  for (uint32_t i = 0; i < kRedo; ++i) {  // a row that is not asked for sees nothing
+    const bool asked = (which >> i & 1u) != 0u;
+    const uint32_t r = asked ? r0 + i : any, token = t.t0 + r / t.stride;
+    row[i] = attend_uniform(attend_row(a, t, r));
+    lo[i] = attend_uniform(attend_begin(a, t.q, token));
+    hi[i] = asked ? attend_uniform(attend_end(t.q, token + 1u)) : 0u;
+    if (hi[i] > lo[i]) {
+      least = lo[i] < least ? lo[i] : least;
+      most = hi[i] > most ? hi[i] : most;
     }
-    s = off == kNoRow ? -__builtin_inff() : s * scale2;
-    const float top = fmaxf(m, seg_allreduce<64>(s, [](float x, float y) { return fmaxf(x, y); }));
-    const float f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-    m = top;
-    const float p = off == kNoRow ? 0.0f : __builtin_amdgcn_exp2f(s - (m == -__builtin_inff() ? 0.0f : m));
-    l = l * f + p;
+    m[i] = -__builtin_inff();
+    l[i] = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= f;
-    for (uint32_t i = 0u; i < 64u && j0 + i < hi; ++i) {
-      const float pi = __shfl(p, static_cast<int>(i), 64);
-      const uint32_t at = __shfl(off, static_cast<int>(i), 64);
-      if (at == kNoRow || lane >= a.D / 4u) continue;
-      const vec<T, 4> x = load_vec<T, 4>(v + static_cast<uint64_t>(at) * 8u + lane * 4u);
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+  }
+  for (uint32_t j0 = least; j0 < most; j0 += 64u) {
+    const uint32_t j = j0 + lane, off = attend_key(a, t, j, least, most);
+    float p[kRedo] = {};
+    if (off != kNoRow) {
+#pragma unroll 2
+      for (uint32_t c = 0u; c < D8; ++c) {
+        const vec<T, 8> y = __builtin_bit_cast(vec<T, 8>, reinterpret_cast<const uint4*>(k)[static_cast<uint64_t>(off) + c]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += pi * static_cast<float>(x[e]);
+        for (uint32_t i = 0; i < kRedo; ++i) {
+          const vec<T, 8> x = __builtin_bit_cast(vec<T, 8>, reinterpret_cast<const uint4*>(q)[static_cast<uint64_t>(row[i]) * D8 + c]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p[i] = fmaf(static_cast<float>(x[e]), static_cast<float>(y[e]), p[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kRedo; ++i) {
+      const bool sees = off != kNoRow && j >= lo[i] && j < hi[i];
+      const float s = sees ? p[i] * scale2 : -__builtin_inff();
+      const float top = fmaxf(m[i], seg_allreduce<64>(s, [](float x, float y) { return fmaxf(x, y); }));
+      const float f = m[i] == top ? 1.0f : __builtin_amdgcn_exp2f(m[i] - top);
+      m[i] = top;
+      p[i] = sees ? __builtin_amdgcn_exp2f(s - (top == -__builtin_inff() ? 0.0f : top)) : 0.0f;
+      l[i] = l[i] * f + p[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] *= f;
+    }
+    constexpr uint32_t kAhead = 8u;
+    for (uint32_t n = 0u; n < 64u && j0 + n < most; n += kAhead) {
+      vec<T, 4> x[kAhead];
+#pragma unroll
+      for (uint32_t u = 0; u < kAhead; ++u) {
+        const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(off), static_cast<int>(n + u)));
+        x[u] = vec<T, 4>{};
+        if (at != kNoRow && lane < a.D / 4u) x[u] = load_vec<T, 4>(v + static_cast<uint64_t>(at) * 8u + lane * 4u);
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < kAhead; ++u) {
+#pragma unroll
+        for (uint32_t i = 0; i < kRedo; ++i) {
+          const float w = __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(p[i])), static_cast<int>(n + u))));
+          if (j0 + n + u < lo[i] || j0 + n + u >= hi[i]) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] += w * static_cast<float>(x[u][e]);
+        }
+      }
     }
   }
-  l = seg_allreduce<64>(l, [](float x, float y) { return x + y; });
-  const float g = l == 0.0f ? 0.0f : 1.0f / l;
-  if (lane < a.D / 4u) {
-    vec<T, 4> w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w.set(e, static_cast<T>(o[e] * g));
-    store_vec<T, 4>(out.y + static_cast<uint64_t>(row) * a.D + lane * 4u, w);
+  for (uint32_t i = 0; i < kRedo; ++i) {
+    l[i] = seg_allreduce<64>(l[i], [](float x, float y) { return x + y; });
+    if ((which >> i & 1u) == 0u) continue;
+    const float g = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+    if (lane < a.D / 4u) {
+      vec<T, 4> w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w.set(e, static_cast<T>(o[i][e] * g));
+      store_vec<T, 4>(out.y + static_cast<uint64_t>(row[i]) * a.D + lane * 4u, w);
+    }
+    if (lane == 0u && out.lse != nullptr) out.lse[row[i]] = l[i] == 0.0f ? -__builtin_inff() : (m[i] + __builtin_log2f(l[i])) * kLn2;
   }
-  if (lane == 0u && out.lse != nullptr) out.lse[row] = l == 0.0f ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2;
 }
 // The rows of the tiles that a flagged workgroup has units of, but those of one
-// position: those that are not finite are done again, the others stay as their sums
-// (or the join of their parts) have them.
+// position: those that a value which they do not see has got into are done again, the
+// others stay as their sums (or the join of their parts) have them. So a sequence of NaN
+// costs a look at each of its tiles, and its first NaN the rows before it in a tile: f16
+// prompts of 4096 take 0.42 ms, 0.65 with a NaN at the first token, 5.8 at the last (54
+// and 17 where each row that is not finite was done again).
 template <bool F16, uint32_t DP, bool MANY, typename T>
-__device__ __forceinline__ void redo_rows(const AttendShape& a, const AttendCount& c, const AttendOut<T>& out, const T* q, const T* k, const T* v,
-                                          float scale2) {
+__device__ __forceinline__ void redo_rows(const AttendShape& a, const AttendCount& c, AttendOdd* odd, const AttendOut<T>& out, const T* q, const T* k,
+                                          const T* v, float scale2) {
   const uint32_t slices = gridDim.x / kAttendGroups, g = blockIdx.x / slices, slice = blockIdx.x % slices;
   if (out.join[8u * g + 7u] == 0u) return;
   const uint64_t units = c.before[MANY ? 1 : 0][256], run = attend_run(units), begin = run * g;
@@ -1270,27 +1365,33 @@ __device__ __forceinline__ void redo_rows(const AttendShape& a, const AttendCoun
   if (begin >= end) return;
   AttendTile t = attend_tile<MANY, DP>(a, c, begin);
   for (;;) {
-    const uint32_t rows = (t.t1 - t.t0) * t.stride, lane = threadIdx.x & 63u;
+    const uint32_t rows = t.t1 - t.t0 > 1u ? (t.t1 - t.t0) * t.stride : 0u, lane = threadIdx.x & 63u;
     const AttendPlace place = attend_place_of(t);
     const uint32_t from = static_cast<uint32_t>(t.first / run), parts = static_cast<uint32_t>((t.end - 1u) / run) - from + 1u;
-    for (uint32_t r = slice * 4u + (threadIdx.x >> 6); t.t1 - t.t0 > 1u && r < rows; r += 4u * slices) {
-      const uint32_t row = place.row(a, r);
-      if (row == kNoRow) continue;
-      JoinSum s;
-      if (lane < a.D / 4u) {
-        if (parts > 1u) {
-          s.all(out, a.D, from, parts, r, lane * 4u);
-        } else {
-          const vec<T, 4> x = load_vec<T, 4>(out.y + static_cast<uint64_t>(row) * a.D + lane * 4u);
+    if (rows != 0u) attend_find_odd(a, t, v, odd);
+    for (uint32_t r0 = (slice * 4u + (threadIdx.x >> 6)) * kRedo; r0 < rows; r0 += 4u * kRedo * slices) {
+      uint32_t which = 0u;
+      for (uint32_t i = 0u; i < kRedo && r0 + i < rows; ++i) {
+        const uint32_t row = place.row(a, r0 + i), token = t.t0 + (r0 + i) / t.stride;
+        if (row == kNoRow) continue;
+        const uint32_t lo = attend_begin(a, t.q, token), hi = attend_end(t.q, token + 1u);
+        JoinSum s;
+        bool off = false;
+        if (lane < a.D / 4u) {
+          if (parts > 1u) {
+            s.all(out, a.D, from, parts, r0 + i, lane * 4u);
+          } else {
+            const vec<T, 4> x = load_vec<T, 4>(out.y + static_cast<uint64_t>(row) * a.D + lane * 4u);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s.o[e] = static_cast<float>(x[e]);
+            for (int e = 0; e < 4; ++e) s.o[e] = static_cast<float>(x[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) off |= !(s.o[e] - s.o[e] == 0.0f) && attend_off(*odd, lane * 4u + e, lo, hi);
         }
+        if (__builtin_amdgcn_ballot_w64(off) != 0u) which |= 1u << i;
+        else if (parts > 1u && lane < a.D / 4u) attend_store<F16>(a, place, out, -1, r0 + i, lane * 4u, s.o, s.m, s.l);
       }
-      float z = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) z += s.o[e] - s.o[e];
-      if (__builtin_amdgcn_ballot_w64(!(z == 0.0f)) != 0u) redo_row<F16>(a, t, r, out, q, k, v, scale2, lane);
-      else if (parts > 1u && lane < a.D / 4u) attend_store<F16>(a, place, out, -1, r, lane * 4u, s.o, s.m, s.l);
+      if (which != 0u) redo_some<F16>(a, t, r0, which, out, q, k, v, scale2, lane);
     }
     if (t.end >= end) break;
     attend_next<MANY, DP>(a, c, t);
@@ -1305,9 +1406,10 @@ __device__ __forceinline__ void join_attention(const AttendShape& a, const T* q,
   const uint32_t g = blockIdx.x / (gridDim.x / kAttendGroups);
   if ((many.join[8u * g + 7u] | few.join[8u * g + 7u]) == 0u) return;
   __shared__ AttendCount c;
+  __shared__ AttendOdd odd;
   attend_count<DP>(a, &c);
-  redo_rows<F16, DP, true>(a, c, many, q, k, v, scale * kLog2e);
-  redo_rows<F16, DP, false>(a, c, few, q, k, v, scale * kLog2e);
+  redo_rows<F16, DP, true>(a, c, &odd, many, q, k, v, scale * kLog2e);
+  redo_rows<F16, DP, false>(a, c, &odd, few, q, k, v, scale * kLog2e);
 }
 
 }  // namespace hip

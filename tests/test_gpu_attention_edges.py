@@ -320,3 +320,89 @@ def test_values_that_are_not_finite_in_any_tile(gpu, name, bad):
     rest = torch.ones(D, dtype=torch.bool, device="cuda")
     rest[D // 2] = False
     close(y[:n][hit[:n]][..., rest], want[0][:n][hit[:n]][..., rest], want[2][:n][hit[:n]][..., rest], "other columns of rows that see it")
+
+
+def spoil(case, s, i, h, d, value):
+    """Puts a value of new token i of sequence s, key head h, column d (or all) into the cache."""
+    _, _, v, table, starts, lens = case
+    at = lens[s] - (starts[s + 1] - starts[s]) + i
+    page = case[1].shape[2]
+    v[int(table[s, at // page]), h, at % page, d] = value
+
+
+@pytest.mark.parametrize("elem", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [128, 256])
+def test_infinite_values_before_nan(gpu, elem, D):
+    """Rows between an infinite value and a NaN of the same column see the first alone,
+    those behind both have NaN; -inf and inf make NaN where both are seen."""
+    n = 300
+    case = make(gen_of("inf nan", D, elem), elem, [n + 37], [n], 2, 2, D, 16)
+    for i, d, value in ((20, 3, "inf"), (40, 3, "nan"), (50, 5, "-inf"), (90, 5, "inf"), (100, 7, "nan"), (270, 7, "inf"), (0, 9, "-inf"), (299, 9, "nan")):
+        spoil(case, 0, i, 1, d, float(value))
+    y, lse = run(elem, case, D ** -0.5)
+    want, wl, by, bl = ref.paged_attention(*case, D ** -0.5, 0, DTYPES[elem])
+    close(lse, wl, bl, "the statistics, which no value enters")
+    for d, spans in ((3, ((0, 20, None), (20, 40, "inf"), (40, n, "nan"))), (5, ((0, 50, None), (50, 90, "-inf"), (90, n, "nan"))),
+                     (7, ((0, 100, None), (100, n, "nan"))), (9, ((0, 299, "-inf"), (299, n, "nan")))):
+        for a, b, value in spans:
+            got = y[a:b, 1, :, d]
+            if value == "nan":
+                assert got.isnan().all(), (d, a)
+            elif value:
+                assert (got == float(value)).all(), (d, a)
+            else:
+                # the reference's products of 0 and what is not finite are NaN: without it
+                clean = [t.clone() if t is case[2] else t for t in case]
+                clean[2] = clean[2].nan_to_num(0.0, 0.0, 0.0)
+                cy, _, cb, _ = ref.paged_attention(*clean, D ** -0.5, 0, DTYPES[elem])
+                close(got, cy[a:b, 1, :, d], cb[a:b, 1, :, d], "rows before it")
+    rest = torch.ones(D, dtype=torch.bool, device="cuda")
+    rest[[3, 5, 7, 9]] = False
+    close(y[..., rest], want[..., rest], by[..., rest], "other columns")
+    close(y[:, 0], want[:, 0], by[:, 0], "the other head")
+
+
+@pytest.mark.parametrize("window", [0, 40, 700])
+def test_a_sequence_of_nan(gpu, window):
+    """One of three sequences holds nothing but NaN values: its rows are NaN, the others as without it."""
+    case = make(gen_of("all nan", window), "bf16", [900, 1300, 500], [300, 1000, 4], 2, 4, 64, 16)
+    want = ref.paged_attention(*case, 0.125, window, DTYPES["bf16"])
+    q, k, v, table, starts, _ = case
+    v[table[1][table[1] >= 0].long()] = float("nan")
+    y, lse = run("bf16", case, 0.125, window)
+    mine = torch.zeros(q.shape[0], dtype=torch.bool, device="cuda")
+    mine[starts[1]:starts[2]] = True
+    assert y[mine].isnan().all()
+    close(y[~mine], want[0][~mine], want[2][~mine], "the others")
+    close(lse, want[1], want[3], "the statistics")
+
+
+def test_values_that_are_not_finite_cost_little(gpu):
+    """A prompt with a NaN at its first token or in all of them: a launch takes not many
+    times as long as without (each row that saw one went through its keys again, by
+    itself: 130 times). Rows of a tile that do not see a NaN of its do that still."""
+    def took(case):
+        q, k, v, table, starts, lens = case
+        p = program(attention.paged_attention, "bf16")
+        tensors = [q, k, v, table, ints(starts), ints(lens), torch.empty_like(q)]
+        best = float("inf")
+        for i in range(6):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            p.launch(tensors, scalars=(0.1,))
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b)) if i else best
+        return best
+    n = 4096
+    case = make(gen_of("cost"), "bf16", [n], [n], 8, 4, 128, 64)
+    clean = took(case)
+    for what, tokens, most in (("first", [0], 12), ("all", range(n), 12)):
+        spoilt = [t.clone() if t is case[2] else t for t in case]
+        for i in (tokens if what != "all" else ()):
+            spoil(spoilt, 0, i, slice(None), slice(None), float("nan"))
+        if what == "all":
+            spoilt[2].fill_(float("nan"))
+        t = took(spoilt)
+        print("NaN at %s: %.3f ms, %.3f without" % (what, t, clean), flush=True)
+        assert t <= most * clean
