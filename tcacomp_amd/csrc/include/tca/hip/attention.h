@@ -412,12 +412,12 @@ __device__ __forceinline__ void attend_load_q(AttendQ<DP>& q, const uint4* __res
   }
 }
 
-// The state of QT x 32 rows: O^T, the reference of the exponents (log2), the
-// lane's part of the sum.
-template <uint32_t DP, int QT>
+// The state of 32 rows: O^T, the reference of the exponents (log2), the lane's part
+// of the sum.
+template <uint32_t DP>
 struct AttendAcc {
-  f32x16 o[QT][DP / 32u];
-  float m[QT], l[QT];
+  f32x16 o[DP / 32u];
+  float m, l;
 };
 
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
@@ -432,18 +432,15 @@ constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 template <bool F16>
 constexpr float kBoost = F16 ? 6.0f : 0.0f;
 
-// One block of KT x 32 keys for QT x 32 rows. `seen(kt)`: which of 32 keys have a
-// row (bits); whole: every key is seen by every row.
-template <bool F16, uint32_t DP, int QT, int KT>
-__device__ __forceinline__ void attend_scores(f32x16 (&s)[KT][QT], const AttendQ<DP> (&q)[QT], const uint16_t* k, uint32_t lane) {
+// Scores of KT x 32 keys for 32 rows.
+template <bool F16, uint32_t DP, int KT>
+__device__ __forceinline__ void attend_scores(f32x16 (&s)[KT], const AttendQ<DP>& q, const uint16_t* k, uint32_t lane) {
   using L = AttendLds<DP>;
   const uint32_t row = lane & 31u, h = lane >> 5;
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[kt][qt][i] = 0.0f;
+    for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
   // Operands are read a group of chunks ahead of the products that take them.
   constexpr uint32_t C = 2u, N = DP / 16u / C;
   bf16x8 f[2][C][KT];
@@ -465,9 +462,7 @@ __device__ __forceinline__ void attend_scores(f32x16 (&s)[KT][QT], const AttendQ
 #pragma unroll
     for (uint32_t c = 0; c < C; ++c)
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) s[kt][qt] = mfma_32x32x16<F16>(f[g & 1u][c][kt], q[qt].v[g * C + c], s[kt][qt]);
+      for (int kt = 0; kt < KT; ++kt) s[kt] = mfma_32x32x16<F16>(f[g & 1u][c][kt], q.v[g * C + c], s[kt]);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -482,81 +477,79 @@ __device__ __forceinline__ float attend_halves_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Scores to probabilities, in 16 bits: p[kt][qt][m] is the B operand of keys 16 m .. 16 m + 15.
-template <bool F16, uint32_t DP, int QT, int KT>
-__device__ __forceinline__ void attend_softmax(const f32x16 (&s)[KT][QT], bf16x8 (&p)[KT][QT][2], AttendAcc<DP, QT>& acc, float scale2,
-                                               bool whole, const uint32_t (&seen)[KT], uint32_t key0, const int32_t (&pos)[QT],
+// Scores to probabilities, in 16 bits: p[kt][m] is the B operand of keys 16 m .. 16 m + 15.
+// seen[kt]: which of 32 keys have a row (bits); whole: every key is seen by every row.
+template <bool F16, uint32_t DP, int KT>
+__device__ __forceinline__ void attend_softmax(const f32x16 (&s)[KT], bf16x8 (&p)[KT][2], AttendAcc<DP>& acc, float scale2,
+                                               bool whole, const uint32_t (&seen)[KT], uint32_t key0, int32_t pos,
                                                uint32_t window, uint32_t lane) {
   const uint32_t h = lane >> 5;
+  float v[KT][16];
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    float v[KT][16];
+  for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+    for (int i = 0; i < 16; ++i) v[kt][i] = s[kt][i];
+  if (!whole) {
+    // Key key0 + 4 h + c of the lane's 32 kt + {0..3, 8..11, ..}: constants c against the row's place.
+    int32_t last = pos - static_cast<int32_t>(key0 + 4u * h);
+    asm volatile("" : "+v"(last));  // nothing of this is kept outside of the branch
+    const int32_t before = window == 0u || window > 0x7fffffffu ? -1 : last - static_cast<int32_t>(window);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[kt][i] = s[kt][qt][i];
-    if (!whole) {
-      // Key key0 + 4 h + c of the lane's 32 kt + {0..3, 8..11, ..}: constants c against the row's place.
-      int32_t last = pos[qt] - static_cast<int32_t>(key0 + 4u * h);
-      asm volatile("" : "+v"(last));  // nothing of this is kept outside of the branch
-      const int32_t before = window == 0u || window > 0x7fffffffu ? -1 : last - static_cast<int32_t>(window);
+    for (int kt = 0; kt < KT; ++kt) {
+      const uint32_t bits = seen[kt] >> (4u * h);
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const uint32_t bits = seen[kt] >> (4u * h);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int32_t c = 8 * (i / 4) + i % 4;
-          const bool sees = (bits & (1u << c)) != 0u && 32 * kt + c <= last && 32 * kt + c > before;
-          v[kt][i] = sees ? v[kt][i] : -__builtin_inff();
-        }
+      for (int i = 0; i < 16; ++i) {
+        const int32_t c = 8 * (i / 4) + i % 4;
+        const bool sees = (bits & (1u << c)) != 0u && 32 * kt + c <= last && 32 * kt + c > before;
+        v[kt][i] = sees ? v[kt][i] : -__builtin_inff();
       }
     }
-    float top = v[0][0];
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, v[kt][i]);
-    top = attend_halves_max(top) * scale2;
-    if (__builtin_amdgcn_ballot_w64(top > acc.m[qt] + 8.0f) != 0u) {
-      const float m = fmaxf(acc.m[qt], top);
-      const float f = m == acc.m[qt] ? 1.0f : __builtin_amdgcn_exp2f(acc.m[qt] - m);
-      acc.m[qt] = m;
-      acc.l[qt] *= f;
-#pragma unroll
-      for (uint32_t d = 0; d < DP / 32u; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc.o[qt][d][i] *= f;
-    }
-    const float sh = (acc.m[qt] == -__builtin_inff() ? 0.0f : acc.m[qt]) - kBoost<F16>;
-    float sum = 0.0f;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        if constexpr (F16) {
-          f16x8 w;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(v[kt][8 * m + e], scale2, -sh));
-            sum += x;
-            w[e] = static_cast<_Float16>(x);
-          }
-          p[kt][qt][m] = __builtin_bit_cast(bf16x8, w);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(v[kt][8 * m + e], scale2, -sh));
-            sum += x;
-            p[kt][qt][m][e] = static_cast<__bf16>(x);
-          }
-        }
-      }
-    acc.l[qt] += sum;
   }
+  float top = v[0][0];
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, v[kt][i]);
+  top = attend_halves_max(top) * scale2;
+  if (__builtin_amdgcn_ballot_w64(top > acc.m + 8.0f) != 0u) {
+    const float m = fmaxf(acc.m, top);
+    const float f = m == acc.m ? 1.0f : __builtin_amdgcn_exp2f(acc.m - m);
+    acc.m = m;
+    acc.l *= f;
+#pragma unroll
+    for (uint32_t d = 0; d < DP / 32u; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc.o[d][i] *= f;
+  }
+  const float sh = (acc.m == -__builtin_inff() ? 0.0f : acc.m) - kBoost<F16>;
+  float sum = 0.0f;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      if constexpr (F16) {
+        f16x8 w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(v[kt][8 * m + e], scale2, -sh));
+          sum += x;
+          w[e] = static_cast<_Float16>(x);
+        }
+        p[kt][m] = __builtin_bit_cast(bf16x8, w);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(v[kt][8 * m + e], scale2, -sh));
+          sum += x;
+          p[kt][m][e] = static_cast<__bf16>(x);
+        }
+      }
+    }
+  acc.l += sum;
 }
 
 // O^T += V^T P^T. The operands of 32 columns at a time, read ahead as those of the scores.
-template <bool F16, uint32_t DP, int QT, int KT>
+template <bool F16, uint32_t DP, int KT>
 struct AttendV {
   using L = AttendLds<DP>;
   uint32_t at;
@@ -579,9 +572,8 @@ struct AttendV {
         f[d & 1u][kt][m] = __builtin_bit_cast(bf16x8, w);
       }
   }
-  // read(0) has been called. beside(): what is issued beside the second group of products.
-  template <typename Beside>
-  __device__ __forceinline__ void add(AttendAcc<DP, QT>& acc, const bf16x8 (&p)[KT][QT][2], const Beside& beside) {
+  // read(0) has been called.
+  __device__ __forceinline__ void add(AttendAcc<DP>& acc, const bf16x8 (&p)[KT][2]) {
 #pragma unroll
     for (uint32_t d = 0; d < DP / 32u; ++d) {
       if (d + 1u < DP / 32u) read(d + 1u);
@@ -589,11 +581,8 @@ struct AttendV {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) acc.o[qt][d] = mfma_32x32x16<F16>(f[d & 1u][kt][m], p[kt][qt][m], acc.o[qt][d]);
+        for (int m = 0; m < 2; ++m) acc.o[d] = mfma_32x32x16<F16>(f[d & 1u][kt][m], p[kt][m], acc.o[d]);
       __builtin_amdgcn_sched_barrier(0);
-      if (d == 0u) beside();
     }
   }
 };
@@ -603,12 +592,12 @@ struct AttendV {
 // where rows of different positions share a block, a flag of the workgroup has those
 // that this has happened to done again (redo_rows).
 template <uint32_t DP>
-__device__ __forceinline__ bool attend_odd(const AttendAcc<DP, 1>& acc) {
+__device__ __forceinline__ bool attend_odd(const AttendAcc<DP>& acc) {
   float z = 0.0f;
 #pragma unroll
   for (uint32_t d = 0; d < DP / 32u; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) z += acc.o[0][d][i] - acc.o[0][d][i];
+    for (int i = 0; i < 16; ++i) z += acc.o[d][i] - acc.o[d][i];
   return !(z == 0.0f);
 }
 
@@ -652,7 +641,7 @@ struct AttendPhase {
   // group i. What is issued between two products fits the 32 cycles that one takes:
   // four products and then all else took 1660 cycles for 1024.
   template <bool FIRST, bool LAST, typename Beside>
-  __device__ __forceinline__ void run(AttendAcc<DP, 1>& acc, const bf16x8 (&p)[2][1][2], f32x16 (&s)[2][1], const AttendQ<DP>& q,
+  __device__ __forceinline__ void run(AttendAcc<DP>& acc, const bf16x8 (&p)[2][2], f32x16 (&s)[2], const AttendQ<DP>& q,
                                       const Beside& beside) {
     constexpr uint32_t from = FIRST ? NV : 0u, to = LAST ? NV : N;
     if constexpr (FIRST) {
@@ -666,14 +655,14 @@ struct AttendPhase {
         __builtin_amdgcn_sched_barrier(0);
         if (i < NV) {
           const uint32_t d = i / 2u * 2u + (j & 1u);
-          acc.o[0][d] = mfma_32x32x16<F16>(f[i % 3u][j], p[i & 1u][0][j >> 1], acc.o[0][d]);
+          acc.o[d] = mfma_32x32x16<F16>(f[i % 3u][j], p[i & 1u][j >> 1], acc.o[d]);
         } else {
           const uint32_t c = (i - NV) * 2u + (j >> 1), kt = j & 1u;
           if (c == 0u) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[kt][0][e] = 0.0f;
+            for (int e = 0; e < 16; ++e) s[kt][e] = 0.0f;
           }
-          s[kt][0] = mfma_32x32x16<F16>(f[i % 3u][j], q.v[c], s[kt][0]);
+          s[kt] = mfma_32x32x16<F16>(f[i % 3u][j], q.v[c], s[kt]);
         }
         __builtin_amdgcn_sched_barrier(0);
         if (i + 2u < to) read(i + 2u, j);
@@ -735,7 +724,7 @@ __device__ __forceinline__ void attend_fence_reads() { asm volatile("s_waitcnt l
 
 // ------------------------------------------------------------- few rows
 // At most 32 rows, the keys split over the waves too: each streams 32 keys of a
-// unit through a ring of its own, without a barrier, and the four sums meet in LDS.
+// unit through a ring of its own, without a barrier, and the waves' sums meet in LDS.
 template <uint32_t DP>
 struct FewLds {
   static constexpr uint32_t W = kAttendWaves<DP>;
@@ -763,17 +752,17 @@ __device__ __forceinline__ void attend_few(const AttendShape& a, const AttendTil
   const uint32_t chunks = a.D / 8u;
   const uint32_t hi = attend_end(t.q, t.t1), lo = attend_begin(a, t.q, t.t0);
 
-  AttendQ<DP> qv[1];
-  attend_load_q<DP>(qv[0], q, attend_row(a, t, lane & 31u), chunks, lane);
-  const int32_t pos[1] = {attend_pos(t, lane & 31u)};
+  AttendQ<DP> qv;
+  attend_load_q<DP>(qv, q, attend_row(a, t, lane & 31u), chunks, lane);
+  const int32_t pos = attend_pos(t, lane & 31u);
   const int32_t pos_min = t.q.base + static_cast<int32_t>(t.t0), pos_max = t.q.base + static_cast<int32_t>(t.t1) - 1;
-  AttendAcc<DP, 1> acc;
-  acc.m[0] = -__builtin_inff();
-  acc.l[0] = 0.0f;
+  AttendAcc<DP> acc;
+  acc.m = -__builtin_inff();
+  acc.l = 0.0f;
 #pragma unroll
   for (uint32_t d = 0; d < DP / 32u; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc.o[0][d][i] = 0.0f;
+    for (int i = 0; i < 16; ++i) acc.o[d][i] = 0.0f;
 
   // The rows of the next kSteps steps from step f on.
   auto refill = [&](uint32_t f) {
@@ -796,7 +785,7 @@ __device__ __forceinline__ void attend_few(const AttendShape& a, const AttendTil
     AttendFill<DP, 32u, 1u>(rows + n % kSteps * 32u, 0u, lane).template load<true>(v, zero, k_slot(n) + F::kBlock, chunks, 0u, lane);
   };
   refill(0u);
-  qv[0].turn(sign);
+  qv.turn(sign);
 #pragma unroll
   for (int n = 0; n < F::NS; ++n) {
     fill_k(n);
@@ -805,20 +794,20 @@ __device__ __forceinline__ void attend_few(const AttendShape& a, const AttendTil
   for (uint32_t n = 0; n < steps; ++n) {
     const uint32_t next = n + F::NS, key0 = (first + n) * kFewKeys<DP> + wave * 32u;
     attend_wait<kFlight>();
-    f32x16 s[1][1];
-    attend_scores<F16, DP, 1, 1>(s, qv, k_slot(n), lane);
+    f32x16 s[1];
+    attend_scores<F16, DP, 1>(s, qv, k_slot(n), lane);
     attend_fence_reads();  // the block's reads, before its slot is loaded again
     if (next % kSteps == 0u) refill(next);
     fill_k(next);
     const uint32_t has[1] = {attend_uniform(seen[n % 32u])};
     const bool whole = has[0] == 0xffffffffu && static_cast<int32_t>(key0 + 31u) <= pos_min &&
                        (a.window == 0u || static_cast<int64_t>(key0) + a.window > pos_max);
-    bf16x8 p[1][1][2];
-    attend_softmax<F16, DP, 1, 1>(s, p, acc, scale2, whole, has, key0, pos, a.window, lane);
+    bf16x8 p[1][2];
+    attend_softmax<F16, DP, 1>(s, p, acc, scale2, whole, has, key0, pos, a.window, lane);
     attend_wait<kFlight>();
-    AttendV<F16, DP, 1, 1> vv(k_slot(n) + F::kBlock, lane);
+    AttendV<F16, DP, 1> vv(k_slot(n) + F::kBlock, lane);
     vv.read(0u);
-    vv.add(acc, p, []() {});
+    vv.add(acc, p);
     attend_fence_reads();
     fill_v(next);
   }
@@ -827,16 +816,16 @@ __device__ __forceinline__ void attend_few(const AttendShape& a, const AttendTil
   constexpr uint32_t W = DP + 4u;
   float* sums = reinterpret_cast<float*>(lds);
   float2* ml = reinterpret_cast<float2*>(lds + F::W * 32u * W * 4u);
-  acc.l[0] = attend_halves_sum(acc.l[0]);
+  acc.l = attend_halves_sum(acc.l);
   const uint32_t rows_here = (t.t1 - t.t0) * t.stride;
   if (t.t1 - t.t0 > 1u && (lane & 31u) < rows_here && attend_odd<DP>(acc)) *odd = 1u;
-  if (lane < 32u) ml[wave * 32u + lane] = float2{acc.m[0], acc.l[0]};
+  if (lane < 32u) ml[wave * 32u + lane] = float2{acc.m, acc.l};
 #pragma unroll
   for (uint32_t d = 0; d < DP / 32u; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if ((lane & 31u) < rows_here) *reinterpret_cast<float4*>(sums + (wave * 32u + (lane & 31u)) * W + 32u * d + 8u * i + 4u * (lane >> 5)) =
-          float4{acc.o[0][d][4 * i], acc.o[0][d][4 * i + 1], acc.o[0][d][4 * i + 2], acc.o[0][d][4 * i + 3]};
+          float4{acc.o[d][4 * i], acc.o[d][4 * i + 1], acc.o[d][4 * i + 2], acc.o[d][4 * i + 3]};
   __syncthreads();
   const AttendPlace place = attend_place_of(t);
   const uint32_t count = rows_here * (DP / 4u);
@@ -866,7 +855,6 @@ __device__ __forceinline__ void attend_few(const AttendShape& a, const AttendTil
 template <uint32_t DP>
 struct ManyLds {
   static constexpr uint32_t W = kAttendWaves<DP>;
-  static constexpr int QT = 1;
   static constexpr bool kTwo = W == 8u;  // two waves on a SIMD
   static constexpr int NS = kTwo ? 4 : DP <= 192u ? 3 : 2;
   static constexpr uint32_t kBlock = kManyKeys * DP;
@@ -880,30 +868,25 @@ __device__ __forceinline__ void attend_many(const AttendShape& a, const AttendTi
                                             const uint4* __restrict__ zero, float scale2, uint32_t sign, uint32_t first, uint32_t steps,
                                             unsigned char* lds, uint32_t* odd) {
   using M = ManyLds<DP>;
-  constexpr int QT = M::QT, kLoads = 2 * attend_loads<DP, kManyKeys, M::W>();
+  constexpr int kLoads = 2 * attend_loads<DP, kManyKeys, M::W>();
   constexpr uint32_t kSteps = M::kRows / kManyKeys;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint16_t* ring = reinterpret_cast<uint16_t*>(lds);
   uint32_t* rows = reinterpret_cast<uint32_t*>(lds + M::kRing);
   uint32_t* seen = rows + M::kRows;  // of two times 16 steps
-  const uint32_t chunks = a.D / 8u, mine = wave * 32u * QT, all = (t.t1 - t.t0) * t.stride;
+  const uint32_t chunks = a.D / 8u, mine = wave * 32u, all = (t.t1 - t.t0) * t.stride;
   const uint32_t hi = attend_end(t.q, t.t1), lo = attend_begin(a, t.q, t.t0);
-  AttendQ<DP> qv[QT];
-  int32_t pos[QT];
-  AttendAcc<DP, QT> acc;
+  AttendQ<DP> qv;
+  attend_load_q<DP>(qv, q, attend_row(a, t, mine + (lane & 31u)), chunks, lane);
+  const int32_t pos = attend_pos(t, mine + (lane & 31u));
+  AttendAcc<DP> acc;
+  acc.m = -__builtin_inff();
+  acc.l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < QT; ++i) {
-    const uint32_t r = mine + 32u * i + (lane & 31u);
-    attend_load_q<DP>(qv[i], q, attend_row(a, t, r), chunks, lane);
-    pos[i] = attend_pos(t, r);
-    acc.m[i] = -__builtin_inff();
-    acc.l[i] = 0.0f;
+  for (uint32_t d = 0; d < DP / 32u; ++d)
 #pragma unroll
-    for (uint32_t d = 0; d < DP / 32u; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc.o[i][d][e] = 0.0f;
-  }
-  const int32_t pos_min = attend_pos(t, mine), pos_max = attend_pos(t, mine + 32u * QT - 1u);
+    for (int e = 0; e < 16; ++e) acc.o[d][e] = 0.0f;
+  const int32_t pos_min = attend_pos(t, mine), pos_max = attend_pos(t, mine + 31u);
 
   // The rows of kSteps / 2 blocks from f on, in one half of rows[]: looked up, and stored when they have come.
   constexpr uint32_t kLook = M::kRows / 2u / (64u * M::W);
@@ -943,8 +926,8 @@ __device__ __forceinline__ void attend_many(const AttendShape& a, const AttendTi
     __builtin_amdgcn_s_barrier();
     asm volatile("" : : : "memory");
   };
-  f32x16 s[2][QT];
-  bf16x8 p[2][QT][2];
+  f32x16 s[2];
+  bf16x8 p[2][2];
   // Whether any of the wave's rows sees block n.
   auto live = [&](uint32_t n) { return mine < all && static_cast<int32_t>((first + n) * kManyKeys) <= pos_max; };
   auto soften = [&](uint32_t n) {
@@ -952,17 +935,11 @@ __device__ __forceinline__ void attend_many(const AttendShape& a, const AttendTi
     const uint32_t has[2] = {attend_uniform(seen[2u * (n % 32u)]), attend_uniform(seen[2u * (n % 32u) + 1u])};
     const bool whole = (has[0] & has[1]) == 0xffffffffu && static_cast<int32_t>(key0 + kManyKeys - 1u) <= pos_min &&
                        (a.window == 0u || static_cast<int64_t>(key0) + a.window > pos_max);
-    attend_softmax<F16, DP, QT, 2>(s, p, acc, scale2, whole, has, key0, pos, a.window, lane);
+    attend_softmax<F16, DP, 2>(s, p, acc, scale2, whole, has, key0, pos, a.window, lane);
   };
-  auto add = [&](uint32_t n, const auto& beside) {
-    AttendV<F16, DP, QT, 2> vv(block(n) + M::kBlock, lane);
-    vv.read(0u);
-    vv.add(acc, p, beside);
-  };
-  auto nothing = [](uint32_t = 0u) {};
+  auto nothing = [](uint32_t) {};
   refill(0u);
-#pragma unroll
-  for (int i = 0; i < QT; ++i) qv[i].turn(sign);
+  qv.turn(sign);
   __syncthreads();
   if (steps == 0u) {
     // no key at all
@@ -994,7 +971,7 @@ __device__ __forceinline__ void attend_many(const AttendShape& a, const AttendTi
       AttendPhase<F16, DP> phase;
       phase.keys(block(0u), lane);
       fill(2u);
-      phase.template run<true, false>(acc, p, s, qv[0], nothing);
+      phase.template run<true, false>(acc, p, s, qv, nothing);
       turn();
       soften(0u);
       phase.begin(block(0u) + M::kBlock, lane);
@@ -1005,7 +982,7 @@ __device__ __forceinline__ void attend_many(const AttendShape& a, const AttendTi
         phase.keys(block(n), lane);
         uint16_t* to = block(n + 2u);
         __builtin_amdgcn_s_setprio(1);
-        phase.template run<false, false>(acc, p, s, qv[0], [&](uint32_t i) {
+        phase.template run<false, false>(acc, p, s, qv, [&](uint32_t i) {
           if (i < Fill::N) f.template load_one<false>(i, k, zero, to, chunks, wave, lane);
           else if (i < 2u * Fill::N) f.template load_one<true>(i - Fill::N, v, zero, to + M::kBlock, chunks, wave, lane);
         });
@@ -1016,7 +993,7 @@ __device__ __forceinline__ void attend_many(const AttendShape& a, const AttendTi
         phase.begin(block(n) + M::kBlock, lane);
         turn();
       }
-      phase.template run<false, true>(acc, p, s, qv[0], nothing);
+      phase.template run<false, true>(acc, p, s, qv, nothing);
     } else {  // no rows: its loads alone
       fill(2u);
       turn();
@@ -1039,16 +1016,18 @@ __device__ __forceinline__ void attend_many(const AttendShape& a, const AttendTi
       if ((n + M::NS) % (kSteps / 2u) == 0u) refill(n + M::NS);
       fill(n + M::NS - 1u);
       if (live(n)) {
-        attend_scores<F16, DP, QT, 2>(s, qv, block(n), lane);
+        attend_scores<F16, DP, 2>(s, qv, block(n), lane);
         soften(n);
-        add(n, nothing);
+        AttendV<F16, DP, 2> vv(block(n) + M::kBlock, lane);
+        vv.read(0u);
+        vv.add(acc, p);
       }
     }
   }
   attend_wait<0>();  // nothing in flight into LDS that is used again
   __syncthreads();
   const AttendPlace place = attend_place_of(t);
-  acc.l[0] = attend_halves_sum(acc.l[0]);
+  acc.l = attend_halves_sum(acc.l);
   const uint32_t r = mine + (lane & 31u);
   if (t.t1 - t.t0 > 1u && r < all && attend_odd<DP>(acc)) *odd = 1u;
   if (slot >= 0) {
@@ -1056,15 +1035,15 @@ __device__ __forceinline__ void attend_many(const AttendShape& a, const AttendTi
     for (uint32_t d = 0; d < DP / 32u; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float o[4] = {acc.o[0][d][4 * e], acc.o[0][d][4 * e + 1], acc.o[0][d][4 * e + 2], acc.o[0][d][4 * e + 3]};
-        attend_store<F16>(a, place, out, slot, r, 32u * d + 8u * e + 4u * (lane >> 5), o, acc.m[0], acc.l[0]);
+        const float o[4] = {acc.o[d][4 * e], acc.o[d][4 * e + 1], acc.o[d][4 * e + 2], acc.o[d][4 * e + 3]};
+        attend_store<F16>(a, place, out, slot, r, 32u * d + 8u * e + 4u * (lane >> 5), o, acc.m, acc.l);
       }
     return;
   }
   // A lane and lane ^ 32 hold four columns each of every eight of a row: they
   // exchange those of two eights, so that each stores 16 bytes.
   const uint32_t row = place.row(a, r);
-  const float f = acc.l[0] == 0.0f ? 0.0f : 1.0f / acc.l[0];
+  const float f = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
 #pragma unroll
   for (uint32_t d = 0; d < DP / 32u; ++d)
 #pragma unroll
@@ -1073,14 +1052,14 @@ __device__ __forceinline__ void attend_many(const AttendShape& a, const AttendTi
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x[i].set(c, static_cast<T>(acc.o[0][d][4 * (e + i) + c] * f));
+        for (int c = 0; c < 4; ++c) x[i].set(c, static_cast<T>(acc.o[d][4 * (e + i) + c] * f));
       const auto lo = __builtin_amdgcn_permlane32_swap(x[0].w[0], x[1].w[0], false, false);
       const auto hi = __builtin_amdgcn_permlane32_swap(x[0].w[1], x[1].w[1], false, false);
       const uint32_t c = 32u * d + 8u * (e + (lane >> 5));
       if (row != kNoRow && c < a.D)
         *reinterpret_cast<uint4*>(out.y + static_cast<uint64_t>(row) * a.D + c) = uint4{lo[0], hi[0], lo[1], hi[1]};
     }
-  if (row != kNoRow && lane < 32u && out.lse != nullptr) out.lse[row] = attend_lse<F16>(acc.m[0], acc.l[0]);
+  if (row != kNoRow && lane < 32u && out.lse != nullptr) out.lse[row] = attend_lse<F16>(acc.m, acc.l);
 }
 
 // ---------------------------------------------------------------- kernels
