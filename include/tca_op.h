@@ -66,6 +66,7 @@
  *       lens and next are those of all new tokens whatever T is.
  *   rotary                elem=f32|bf16|f16 [interleaved] [inverse]       scalar scale
  *       x [T, H, D], pos [T] i32, freq [F] f32 -> y [T, H, D]             2 F <= D, F <= 512
+ *       (T below 2^26: a launch has less than 2^32 lanes; rotary_cache the same)
  *       pair i < F of a head, (a, b) = x[i], x[F + i] (interleaved: x[2 i], x[2 i + 1]):
  *       scale (a c - b s, b c + a s), c and s of the angle pos freq[i]; features
  *       from 2 F on are copied. inverse: s -> -s, the gradient of x from that of y.

@@ -113,7 +113,7 @@ int tca_rt_event_elapsed_ms(tca_event start, tca_event stop, float* ms);
 int tca_rt_module_load(const char* hsaco_path, tca_module* out);
 int tca_rt_module_unload(tca_module m);
 /* Launch grammar for wave64 (replaces runtime/tca/launch.h:37-58): 1-D grid
- * of >= 1 workgroups, block a multiple of 64 and <= 1024, LDS <= the device's
+ * of >= 1 workgroups, block a multiple of 64 and <= 1024, < 2^32 lanes, LDS <= the device's
  * per-workgroup limit (queried; 160 KiB on gfx950). Host-only check. */
 int tca_rt_validate_launch(uint32_t grid, uint32_t block, uint32_t lds_bytes);
 int tca_rt_launch(tca_module m, const char* kernel, uint32_t grid, uint32_t block,

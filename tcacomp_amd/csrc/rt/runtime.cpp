@@ -91,6 +91,9 @@ int check_geometry(uint32_t grid, uint32_t block, uint32_t lds, int max_threads,
     return fail(TCA_ERR_LAUNCH, "launch: block %u is not a positive multiple of the 64-lane wavefront", block);
   if (block > static_cast<uint32_t>(max_threads))
     return fail(TCA_ERR_LAUNCH, "launch: block %u exceeds the device limit of %d threads", block, max_threads);
+  // The dispatch counts lanes in 32 bits and would run what is left of them modulo 2^32.
+  if (static_cast<uint64_t>(grid) * block > 0xffffffffull)
+    return fail(TCA_ERR_LAUNCH, "launch: %u workgroups of %u lanes are more than 2^32-1 lanes", grid, block);
   if (lds > static_cast<uint32_t>(max_lds))
     return fail(TCA_ERR_LAUNCH, "launch: %u bytes of LDS exceed the device limit of %d", lds, max_lds);
   return TCA_OK;
