@@ -12,15 +12,17 @@
 // lane and one exchange with lane ^ 32, the running maximum and sum are a
 // register each, and the probabilities are already the B operand of O^T = V^T
 // P^T: its k slots of a lane half are keys 4h + {0..3, 8..11} of 16, which the
-// transposing LDS read of V takes in the same order. Nothing but the scores'
-// exponentials passes through the vector ALU.
+// transposing LDS read of V takes in the same order. Only the
+// softmax passes through the vector ALU.
 //
-// One token over 8000 to 16000 keys of 8 heads of 128 (bf16): 20 us and 8 of the join, HBM's
-// 6 us behind a chain of lengths, table, keys; 64 sequences of half as many keys: 273 and
-// 5, 5.8 TB/s. Four chunks of 512 over 8000 to 16000 keys, 8 heads of a group: 400 us and
-// 14, 1.0 PFLOP/s (the matrix cores busy for 49% of the cycles); prompts of 4096 (f16) 385
-// and 14, 0.71. Everything runs once, but rows of a tile that a value which is not finite
-// has got into though they do not see it: without the matrix cores (redo_rows).
+// One token over 8000 to 16000 keys of 8 heads of 128 (bf16): 21-22 us and 8.4-8.8 of the
+// join for HBM's 6; 64 sequences of half as many keys: 272-278 and 6, 5.7 TB/s. Four chunks of
+// 512 over 8000 to 16000 keys, 8 heads of a group: 409-440 us and 16 (the matrix cores busy for
+// 49% of the cycles; calls, whose clocks are higher than a trace's, 413 in all, 0.97 PFLOP/s);
+// prompts of 4096 (f16) 395-406 and 16 (calls 392, 0.70). Heads of 256, one wave a SIMD: as
+// many bytes of single tokens 273-278 and 8, prompts of as many operations 559-567 and 15.
+// Everything runs once, but rows of a tile that a value which is not finite has got into
+// though they do not see it: without the matrix cores (redo_rows).
 //
 // Lengths lie on the GPU, so the launch knows shapes only: every workgroup of
 // a fixed grid reads the lengths, counts the work of all sequences in units
@@ -40,7 +42,9 @@ namespace hip {
 constexpr uint32_t kAttendGroups = 256;  // workgroups: one a CU
 // Rows of a sequence and key head that waves split the keys of. (bf16, 8 key heads of 128: 8
 // sequences of 16 rows over 4000 to 8000 keys 45 us so and 49 as tiles of many rows, of 32
-// rows 49 both, 64 of 4 rows 291 and 288, one of 32 over 16000 36.4 and 36.9.)
+// rows 49 both, 64 of 4 rows 291 and 288, one of 32 over 16000 36.4 and 36.9. Calls of 64
+// sequences with 4, 16, 32 rows 293, 339, 358, with 36, 64, 128, 256 as tiles 357, 364, 383, 518:
+// waves of a tile that have no rows cost nothing while the keys come from HBM.)
 constexpr uint32_t kAttendFew = 32;
 // Waves of a workgroup: two on a SIMD, each the softmax beside the other's matrix
 // products, in 256 registers; one where a wave's sums and queries need more. (One

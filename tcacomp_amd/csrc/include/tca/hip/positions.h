@@ -272,7 +272,8 @@ struct RotaryRow {
 
 // A workgroup takes TOKENS tokens: their angles once, then all of their heads. Bound by
 // HBM: bf16 [8192, 32, 128] 21.0 us (6.4 TB/s), f32 of as many values 43.6 (6.2), heads of
-// 77 with 3 pairs 4.4 TB/s; stores into pages, f16 [4096, 48, 128] 18.2 us (5.5 TB/s).
+// 77 with 3 pairs 4.4 TB/s (their pieces of 16 bytes lie across lines, the 3 pairs and the
+// row's last 7 values move one by one); stores into pages, f16 [4096, 48, 128] 18.2 us (5.5 TB/s).
 template <typename T, bool INTER, bool INVERSE, uint32_t TOKENS>
 __device__ __forceinline__ void rotary(const T* x, const int32_t* pos, const float* freq, T* y, uint32_t Tn, uint32_t H, uint32_t D,
                                        uint32_t F, float scale) {
